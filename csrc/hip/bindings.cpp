@@ -1278,6 +1278,7 @@ namespace pbx {
 void bind_tower(py::module& m);
 void bind_ctr(py::module& m);
 void bind_cross(py::module& m);
+void bind_block(py::module& m);
 void bind_ipc(py::module& m);
 }
 
@@ -1286,6 +1287,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_tower(m);
   bind_ctr(m);
   bind_cross(m);
+  bind_block(m);
   bind_ipc(m);
   m.doc() = "PaddleBox-capability engine: hand-written gfx950 (MI355X) kernels";
   py::class_<SparseSGDConfig>(m, "SparseSGDConfig")

@@ -1,0 +1,330 @@
+// torch glue of the dense-block operators (block_norm.hip, block_fp8.hip):
+// shape checks, allocation and the autograd nodes.  Every entry runs on its
+// tensors' device and that device's current stream; nothing outlives the call
+// but the tensors it returns or saves.
+#include <ATen/hip/HIPContext.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPException.h>
+#include <torch/extension.h>
+
+#include "block_ops.h"
+
+namespace py = pybind11;
+using torch::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace pbx {
+namespace {
+
+using OptTensor = c10::optional<Tensor>;  // an autograd node takes no undefined tensor
+
+#define BK_CHECK(cond, ...) TORCH_CHECK(cond, "pbx block: ", __VA_ARGS__)
+
+// a launch that the runtime refused is reported by the call that made it
+void launched() { C10_HIP_KERNEL_LAUNCH_CHECK(); }
+
+hipStream_t stream_of(const Tensor& t) { return at::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+BlockType block_type(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case torch::kFloat32: return kF32;
+    case torch::kBFloat16: return kBF16;
+    case torch::kFloat16: return kF16;
+    default: BK_CHECK(false, name, " must be float32, bfloat16 or float16, not ", t.scalar_type());
+  }
+  return kF32;
+}
+
+void first_order_only() {
+  BK_CHECK(!at::GradMode::is_enabled(), "the backward pass of this operator cannot be differentiated again");
+}
+
+// [M, D] rows with unit column stride: the tensor itself when it has them (any
+// row stride of at least D), else a contiguous copy
+Tensor rows_of(const Tensor& t, int64_t M, int64_t D) {
+  if (t.dim() == 2 && (D == 1 || t.stride(1) == 1) && (M <= 1 || t.stride(0) >= D)) return t;
+  return t.contiguous().view({M, D});
+}
+int64_t ld_of(const Tensor& t, int64_t M, int64_t D) { return M <= 1 ? D : t.stride(0); }
+
+// ------------------------------------------------------------------ dropout mask
+struct MaskOpts {
+  int64_t thr;  // round(p 2^16)
+  double up;    // scale of a kept value
+  int64_t seed, offset;
+};
+
+MaskArgs mask_args(const MaskOpts& o, const Tensor& seed, const Tensor& like) {
+  MaskArgs m;
+  BK_CHECK(o.thr >= 0 && o.thr <= 65536, "dropout threshold out of range");
+  m.thr = (uint32_t)o.thr;
+  m.up = (float)o.up;
+  m.seed_v = o.seed;
+  m.offset_v = o.offset;
+  if (seed.defined() && o.thr) {
+    BK_CHECK(seed.scalar_type() == torch::kInt64 && seed.numel() == 2 && seed.is_contiguous() &&
+                 seed.device() == like.device(),
+             "a seed tensor is a contiguous int64 [2] = (seed, offset) on the input's device");
+    m.seed = seed.data_ptr<int64_t>();
+  }
+  return m;
+}
+
+class DropoutFn : public torch::autograd::Function<DropoutFn> {
+ public:
+  static Tensor run(const Tensor& x, MaskArgs m) {
+    auto xc = x.contiguous();
+    auto y = torch::empty(x.sizes(), xc.options());
+    launch_dropout(xc.data_ptr(), y.data_ptr(), x.numel(), block_type(x, "x"), m, stream_of(x));
+    launched();
+    return y;
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& seed_t, MaskOpts o, bool grad) {
+    c10::DeviceGuard guard(x.device());
+    const Tensor seed = seed_t.value_or(Tensor());
+    MaskArgs m = mask_args(o, seed, x);
+    Tensor used;
+    if (m.seed && grad) {  // the caller's tensor may have moved on by the time of the backward
+      used = torch::empty({2}, seed.options());
+      m.seed_out = used.data_ptr<int64_t>();
+    }
+    auto y = run(x, m);
+    ctx->save_for_backward({used});
+    ctx->saved_data["thr"] = o.thr;
+    ctx->saved_data["up"] = o.up;
+    ctx->saved_data["seed"] = o.seed;
+    ctx->saved_data["offset"] = o.offset;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_order_only();
+    c10::DeviceGuard guard(g[0].device());
+    const Tensor used = ctx->get_saved_variables()[0];
+    const MaskArgs m = mask_args({ctx->saved_data["thr"].toInt(), ctx->saved_data["up"].toDouble(),
+                                  ctx->saved_data["seed"].toInt(), ctx->saved_data["offset"].toInt()},
+                                 used, g[0]);
+    return {run(g[0], m), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// whether an autograd node will be recorded for these inputs
+bool wants_grad(std::initializer_list<OptTensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const OptTensor& t : ts)
+    if (t.has_value() && t->requires_grad()) return true;
+  return false;
+}
+
+Tensor block_dropout(const Tensor& x, const OptTensor& seed, int64_t thr, double up, int64_t seed_v,
+                     int64_t offset_v) {
+  BK_CHECK(x.is_cuda(), "x must be a GPU tensor");
+  block_type(x, "x");
+  return DropoutFn::apply(x, seed, MaskOpts{thr, up, seed_v, offset_v}, wants_grad({x}));
+}
+
+// ------------------------------------------------------------------ gated residual norm
+struct ResidualOpts {
+  int64_t post, pre, gate_kind;
+  bool sigmoid;
+  double x_scale, y_scale, eps;
+  MaskOpts mask;
+};
+
+class ResidualFn : public torch::autograd::Function<ResidualFn> {
+ public:
+  // inputs: x, y, gate, post_w, post_b, pre_w, pre_b, seed
+  static ResidualArgs args(const ResidualOpts& o, const Tensor& y, int64_t M, int64_t D) {
+    ResidualArgs a;
+    a.M = M;
+    a.D = (int)D;
+    a.post = (int)o.post;
+    a.pre = (int)o.pre;
+    a.gate_kind = (int)o.gate_kind;
+    a.sigmoid = o.sigmoid;
+    a.x_scale = (float)o.x_scale;
+    a.y_scale = (float)o.y_scale;
+    a.eps = (float)o.eps;
+    a.t = block_type(y, "y");
+    return a;
+  }
+  static const float* vec(const Tensor& t, bool wanted, int64_t D, const Tensor& like, const char* name) {
+    if (!wanted) return nullptr;
+    BK_CHECK(t.defined() && t.scalar_type() == torch::kFloat32 && t.dim() == 1 && t.size(0) == D &&
+                 t.is_contiguous() && t.device() == like.device(),
+             name, " must be a contiguous float32 [", D, "] on the input's device");
+    return t.data_ptr<float>();
+  }
+  static void params(ResidualArgs& a, const Tensor& like, const Tensor& gate, const Tensor& post_w,
+                     const Tensor& post_b, const Tensor& pre_w, const Tensor& pre_b) {
+    a.post_w = vec(post_w, a.post != kNormNone, a.D, like, "post_weight");
+    a.post_b = vec(post_b, a.post == kNormLayer, a.D, like, "post_bias");
+    a.pre_w = vec(pre_w, a.pre != kNormNone, a.D, like, "pre_weight");
+    a.pre_b = vec(pre_b, a.pre == kNormLayer, a.D, like, "pre_bias");
+    if (a.gate_kind == kGateChannel) a.gate = vec(gate, true, a.D, like, "gate");
+    if (a.gate_kind == kGateRow) {
+      BK_CHECK(gate.defined() && gate.scalar_type() == torch::kFloat32 && gate.numel() == a.M && gate.is_contiguous() &&
+                   gate.device() == like.device(),
+               "a row gate must be a contiguous float32 with one value for each row, on the input's device");
+      a.gate = gate.data_ptr();
+    }
+    if (a.gate_kind == kGateFull) {
+      BK_CHECK(gate.defined() && gate.scalar_type() == like.scalar_type() && gate.dim() == 2 && gate.size(0) == a.M &&
+                   gate.size(1) == a.D && (a.D == 1 || gate.stride(1) == 1) && gate.device() == like.device(),
+               "a full gate must have y's shape, type and device");
+      a.gate = gate.data_ptr();
+      a.ldg = ld_of(gate, a.M, a.D);
+    }
+  }
+
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& y, const OptTensor& gate_t,
+                               const OptTensor& post_wt, const OptTensor& post_bt, const OptTensor& pre_wt,
+                               const OptTensor& pre_bt, const OptTensor& seed_t, ResidualOpts o, bool any) {
+    c10::DeviceGuard guard(x.device());
+    auto v = [](const OptTensor& t) { return t.value_or(Tensor()); };
+    const Tensor gate = v(gate_t), post_w = v(post_wt), post_b = v(post_bt), pre_w = v(pre_wt), pre_b = v(pre_bt),
+                 seed = v(seed_t);
+    const int64_t D = x.size(-1), M = D ? x.numel() / D : 0;
+    BK_CHECK(M < (int64_t(1) << 31), "too many rows");
+    ResidualArgs a = args(o, y, M, D);
+    a.stream_t = block_type(x, "x");
+    BK_CHECK(a.stream_t == a.t || a.stream_t == kF32, "x must have y's type or float32");
+    BK_CHECK(y.sizes() == x.sizes() && y.device() == x.device(), "x and y must have one shape and device");
+    BK_CHECK(D <= kResidualMaxD, "at most ", kResidualMaxD, " columns, not ", D);
+    const Tensor xr = rows_of(x, M, D), yr = rows_of(y, M, D);
+    Tensor gr = gate;
+    if (o.gate_kind == kGateRow) gr = gate.contiguous();
+    if (o.gate_kind == kGateFull) gr = rows_of(gate, M, D);
+    auto c = [](const Tensor& t) { return t.defined() ? t.contiguous() : t; };
+    if (o.gate_kind == kGateChannel) gr = c(gate);
+    const Tensor pw = c(post_w), pb = c(post_b), qw = c(pre_w), qb = c(pre_b);
+    params(a, yr, gr, pw, pb, qw, qb);
+    a.mask = mask_args(o.mask, seed, x);
+    Tensor r = torch::empty(x.sizes(), x.options().memory_format(c10::MemoryFormat::Contiguous));
+    Tensor h = o.pre ? torch::empty(y.sizes(), y.options().memory_format(c10::MemoryFormat::Contiguous)) : Tensor();
+    Tensor stats, used;
+    if (any) {
+      stats = torch::empty({M, 4}, x.options().dtype(torch::kFloat32));
+      a.stats = stats.data_ptr<float>();
+      if (a.mask.seed) {
+        used = torch::empty({2}, seed.options());
+        a.mask.seed_out = used.data_ptr<int64_t>();
+      }
+    }
+    a.x = xr.data_ptr();
+    a.ldx = ld_of(xr, M, D);
+    a.y = yr.data_ptr();
+    a.ldy = ld_of(yr, M, D);
+    a.r = r.data_ptr();
+    a.h = o.pre ? h.data_ptr() : nullptr;
+    launch_residual_fwd(a, stream_of(x));
+    launched();
+    if (any) {
+      // the copies that were made, or views of the inputs: either way what the kernel read
+      ctx->save_for_backward({xr, yr, gr, pw, pb, qw, qb, used});
+      ctx->saved_data["stats"] = stats;
+      for (auto& kv : std::initializer_list<std::pair<const char*, int64_t>>{
+               {"post", o.post}, {"pre", o.pre}, {"gk", o.gate_kind}, {"sig", (int64_t)o.sigmoid},
+               {"thr", o.mask.thr}, {"seed", o.mask.seed}, {"off", o.mask.offset}})
+        ctx->saved_data[kv.first] = kv.second;
+      ctx->saved_data["xs"] = o.x_scale;
+      ctx->saved_data["ys"] = o.y_scale;
+      ctx->saved_data["up"] = o.mask.up;
+      ctx->saved_data["shape"] = x.sizes().vec();
+      ctx->saved_data["gs"] = gate.defined() ? c10::IValue(gate.sizes().vec()) : c10::IValue(std::vector<int64_t>{});
+    }
+    ctx->set_materialize_grads(false);
+    if (o.pre) return {r, h};
+    return {r};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_order_only();
+    const auto sv = ctx->get_saved_variables();
+    auto& sd = ctx->saved_data;
+    const Tensor &x = sv[0], &y = sv[1], &gate = sv[2], &post_w = sv[3], &post_b = sv[4], &pre_w = sv[5],
+                 &pre_b = sv[6], &used = sv[7];
+    c10::DeviceGuard guard(x.device());
+    ResidualOpts o{sd["post"].toInt(), sd["pre"].toInt(), sd["gk"].toInt(), sd["sig"].toInt() != 0, sd["xs"].toDouble(),
+                   sd["ys"].toDouble(), 0.0, {sd["thr"].toInt(), sd["up"].toDouble(), sd["seed"].toInt(), sd["off"].toInt()}};
+    const auto shape = sd["shape"].toIntVector();
+    const int64_t M = x.size(0), D = x.size(1);
+    ResidualArgs a = args(o, y, M, D);
+    a.stream_t = block_type(x, "x");
+    params(a, y, gate, post_w, post_b, pre_w, pre_b);
+    a.mask = mask_args(o.mask, used, x);
+    const Tensor stats = sd["stats"].toTensor();
+    a.stats = stats.data_ptr<float>();
+    a.x = x.data_ptr();
+    a.ldx = ld_of(x, M, D);
+    a.y = y.data_ptr();
+    a.ldy = ld_of(y, M, D);
+    Tensor dr, dh;
+    if (g[0].defined()) {
+      dr = rows_of(g[0], M, D);
+      a.dr = dr.data_ptr();
+      a.lddr = ld_of(dr, M, D);
+    }
+    if (o.pre && g[1].defined()) {
+      dh = rows_of(g[1], M, D);
+      a.dh = dh.data_ptr();
+      a.lddh = ld_of(dh, M, D);
+    }
+    // edges: the tensor arguments that forward() got, in order, without the absent ones
+    const bool have[7] = {true, true, gate.defined(), post_w.defined(), post_b.defined(), pre_w.defined(), pre_b.defined()};
+    auto want = [&](int i) {
+      if (!have[i]) return false;
+      int edge = 0;
+      for (int j = 0; j < i; ++j) edge += have[j];
+      return ctx->needs_input_grad(edge);
+    };
+    auto like_x = x.options(), like_y = y.options(), f32 = x.options().dtype(torch::kFloat32);
+    variable_list out(10);
+    if (want(0)) a.dx = (out[0] = torch::empty(shape, like_x)).data_ptr();
+    if (want(1)) a.dy = (out[1] = torch::empty(shape, like_y)).data_ptr();
+    if (want(2)) {
+      out[2] = torch::empty(sd["gs"].toIntVector(), o.gate_kind == kGateFull ? like_y : f32);
+      a.dgate = out[2].data_ptr();
+    }
+    float** vecs[4] = {&a.dpost_w, &a.dpost_b, &a.dpre_w, &a.dpre_b};
+    for (int i = 0; i < 4; ++i)
+      if (want(3 + i)) *vecs[i] = (out[3 + i] = torch::empty({D}, f32)).data_ptr<float>();
+    if (M == 0) {  // no row: the sums over rows are zero
+      for (auto& t : out)
+        if (t.defined()) t.zero_();
+      return out;
+    }
+    Tensor slab;
+    if (const int nvec = residual_nvec(a)) {
+      slab = torch::empty({(int64_t)residual_slab_rows(M, (int)D), nvec, D}, f32);
+      a.slab = slab.data_ptr<float>();
+    }
+    launch_residual_bwd(a, stream_of(x));
+    launched();
+    return out;
+  }
+};
+
+std::vector<Tensor> block_residual(const Tensor& x, const Tensor& y, const OptTensor& gate,
+                                   const OptTensor& post_w, const OptTensor& post_b,
+                                   const OptTensor& pre_w, const OptTensor& pre_b,
+                                   const OptTensor& seed, int64_t post, int64_t pre, int64_t gate_kind,
+                                   bool sigmoid, double x_scale, double y_scale, double eps, int64_t thr,
+                                   double up, int64_t seed_v, int64_t offset_v) {
+  BK_CHECK(x.is_cuda() && y.is_cuda(), "x and y must be GPU tensors");
+  BK_CHECK(x.dim() >= 1, "x must have at least one dimension");
+  BK_CHECK(post >= 0 && post <= 2 && pre >= 0 && pre <= 2 && gate_kind >= 0 && gate_kind <= 3, "unknown kind");
+  return ResidualFn::apply(
+      x, y, gate, post_w, post_b, pre_w, pre_b, seed,
+      ResidualOpts{post, pre, gate_kind, sigmoid, x_scale, y_scale, eps, {thr, up, seed_v, offset_v}},
+      wants_grad({x, y, gate, post_w, post_b, pre_w, pre_b}));
+}
+
+}  // namespace
+
+void bind_block(py::module_& m) {
+  m.def("block_dropout", &block_dropout);
+  m.def("block_residual", &block_residual);
+}
+
+}  // namespace pbx
