@@ -320,11 +320,245 @@ std::vector<Tensor> block_residual(const Tensor& x, const Tensor& y, const OptTe
       wants_grad({x, y, gate, post_w, post_b, pre_w, pre_b}));
 }
 
+// ------------------------------------------------------------------ 8-bit fc
+constexpr int64_t kFp8MaxDim = 65535 * 128;  // tiles of 128 in a launch's second dimension
+
+void fp8_dims(int64_t a, int64_t b) {
+  BK_CHECK(a <= kFp8MaxDim && b <= kFp8MaxDim, "fp8: at most ", kFp8MaxDim, " rows or columns");
+}
+
+// codes and exponent bytes of a [rows, K] matrix in one allocation
+struct Fp8Buf {
+  Tensor mem;
+  int64_t rows = 0, K = 0;
+  uint8_t* codes() const { return mem.data_ptr<uint8_t>(); }
+  uint8_t* scales() const { return codes() + rows * fp8_kp(K); }
+};
+Fp8Buf fp8_buf(Tensor mem, int64_t rows, int64_t K) { return {mem, rows, K}; }
+Fp8Buf fp8_new(int64_t rows, int64_t K, const Tensor& like) {
+  return {torch::empty({rows * (fp8_kp(K) + fp8_sp(K))}, like.options().dtype(torch::kUInt8)), rows, K};
+}
+
+Fp8QuantArgs quant_args(const Tensor& x, int64_t M, int64_t K, bool tile) {
+  Fp8QuantArgs q;
+  q.x = x.data_ptr();
+  q.t = block_type(x, "x");
+  q.M = M;
+  q.K = K;
+  q.ld = ld_of(x, M, K);
+  q.tile = tile;
+  return q;
+}
+
+void fp8_product(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t* sb, int64_t M, int64_t N,
+                 int64_t K, const float* bias, const Tensor& c) {
+  Fp8GemmArgs g;
+  g.a = a;
+  g.sa = sa;
+  g.b = b;
+  g.sb = sb;
+  g.M = (int)M;
+  g.N = (int)N;
+  g.K = K;
+  g.bias = bias;
+  g.c = c.data_ptr();
+  g.ct = block_type(c, "the result");
+  g.ksplit = fp8_gemm_ksplit(g.M, g.N, K);
+  Tensor slab;
+  if (g.ksplit > 1) {
+    slab = torch::empty({(int64_t)g.ksplit, M, N}, c.options().dtype(torch::kFloat32));
+    g.slab = slab.data_ptr<float>();
+  }
+  launch_fp8_gemm(g, stream_of(c));
+  launched();
+}
+void fp8_product(const Fp8Buf& a, const Fp8Buf& b, const float* bias, const Tensor& c) {
+  fp8_product(a.codes(), a.scales(), b.codes(), b.scales(), a.rows, b.rows, a.K, bias, c);
+}
+
+const float* bias_of(const Tensor& b, int64_t N, const Tensor& like) {
+  if (!b.defined()) return nullptr;
+  BK_CHECK(b.scalar_type() == torch::kFloat32 && b.numel() == N && b.is_contiguous() && b.device() == like.device(),
+           "a bias is a contiguous float32 [", N, "] on the input's device");
+  return b.data_ptr<float>();
+}
+
+// x [M, K] -> (codes, scales) in blocks along K, or of x^T in blocks along M
+std::vector<Tensor> block_fp8_quantize(const Tensor& x, bool tile, bool transposed) {
+  BK_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) > 0, "x must be a GPU matrix");
+  c10::DeviceGuard guard(x.device());
+  const int64_t M = x.size(0), K = x.size(1);
+  fp8_dims(M, K);
+  const Tensor xr = rows_of(x.detach(), M, K);
+  auto q = quant_args(xr, M, K, tile);
+  const int64_t rows = transposed ? K : M, cols = transposed ? M : K;
+  auto codes = torch::empty({rows, fp8_kp(cols)}, x.options().dtype(torch::kFloat8_e4m3fn));
+  auto scales = torch::empty({rows, fp8_sp(cols)}, x.options().dtype(torch::kUInt8));
+  uint8_t* c = reinterpret_cast<uint8_t*>(codes.data_ptr());
+  (transposed ? q.col_codes : q.row_codes) = c;
+  (transposed ? q.col_scales : q.row_scales) = scales.data_ptr<uint8_t>();
+  launch_fp8_quant(q, stream_of(x));
+  launched();
+  return {codes, scales};
+}
+
+void check_blocks(const Tensor& codes, const Tensor& scales, int64_t K, const char* name) {
+  BK_CHECK(codes.is_cuda() && codes.scalar_type() == torch::kFloat8_e4m3fn && codes.dim() == 2 && codes.is_contiguous() &&
+               codes.size(1) == fp8_kp(K) && reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 == 0,
+           name, " codes must be a contiguous float8_e4m3fn [rows, ", fp8_kp(K), "] at a 16-byte address");
+  BK_CHECK(scales.device() == codes.device() && scales.scalar_type() == torch::kUInt8 && scales.dim() == 2 &&
+               scales.is_contiguous() && scales.size(0) == codes.size(0) && scales.size(1) == fp8_sp(K) &&
+               reinterpret_cast<uintptr_t>(scales.data_ptr()) % 4 == 0,
+           name, " scales must be a contiguous uint8 [rows, ", fp8_sp(K), "] beside the codes");
+  fp8_dims(codes.size(0), K);
+}
+const uint8_t* bytes(const Tensor& t) { return reinterpret_cast<const uint8_t*>(t.data_ptr()); }
+
+Tensor block_fp8_matmul(const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, int64_t K,
+                        const OptTensor& bias, at::ScalarType out) {
+  check_blocks(a, sa, K, "a");
+  check_blocks(b, sb, K, "b");
+  BK_CHECK(a.device() == b.device(), "a and b must be on one device");
+  c10::DeviceGuard guard(a.device());
+  const Tensor bc = bias.has_value() ? bias->detach().contiguous() : Tensor();
+  auto c = torch::empty({a.size(0), b.size(0)}, a.options().dtype(out));
+  fp8_product(bytes(a), bytes(sa), bytes(b), bytes(sb), a.size(0), b.size(0), K, bias_of(bc, b.size(0), a), c);
+  return c;
+}
+
+// y = q(x) q(W) + b with a packed weight (codes of W^T)
+Tensor block_fp8_fc_packed(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& b) {
+  BK_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) > 0, "x must be a GPU matrix");
+  check_blocks(codes, scales, x.size(1), "weight");
+  BK_CHECK(codes.device() == x.device(), "x and the weight must be on one device");
+  c10::DeviceGuard guard(x.device());
+  const int64_t M = x.size(0), K = x.size(1), O = codes.size(0);
+  fp8_dims(M, O);
+  const Tensor xr = rows_of(x.detach(), M, K), bc = b.has_value() ? b->detach().contiguous() : Tensor();
+  auto q = quant_args(xr, M, K, false);
+  const Fp8Buf xq = fp8_new(M, K, x);
+  q.row_codes = xq.codes();
+  q.row_scales = xq.scales();
+  launch_fp8_quant(q, stream_of(x));
+  launched();
+  auto y = torch::empty({M, O}, x.options().memory_format(c10::MemoryFormat::Contiguous));
+  fp8_product(xq.codes(), xq.scales(), bytes(codes), bytes(scales), M, O, K, bias_of(bc, O, x), y);
+  return y;
+}
+
+// Training: x and dy are held in blocks along K / O for the forward and dx
+// and, from the same read, in blocks along the batch for dW; W in 128 x 128
+// blocks, whose codes serve the forward and dx alike.  What the backward keeps
+// is 8 bits a value: x^T's codes and W's.
+class Fp8FcFn : public torch::autograd::Function<Fp8FcFn> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& W, const OptTensor& b, bool grad) {
+    c10::DeviceGuard guard(x.device());
+    const int64_t M = x.size(0), K = x.size(1), O = W.size(1);
+    const Tensor xr = rows_of(x, M, K), Wr = rows_of(W, K, O), bc = b.has_value() ? b->contiguous() : Tensor();
+    const bool need_dx = grad && x.requires_grad(), need_dw = grad && W.requires_grad();
+    auto s = stream_of(x);
+    const Fp8Buf wt = fp8_new(O, K, x), xq = fp8_new(M, K, x);
+    Fp8Buf wq, xt;
+    auto qw = quant_args(Wr, K, O, true);
+    qw.col_codes = wt.codes();
+    qw.col_scales = wt.scales();
+    if (need_dx) {
+      wq = fp8_new(K, O, x);
+      qw.row_codes = wq.codes();
+      qw.row_scales = wq.scales();
+    }
+    launch_fp8_quant(qw, s);
+    auto qx = quant_args(xr, M, K, false);
+    qx.row_codes = xq.codes();
+    qx.row_scales = xq.scales();
+    if (need_dw) {
+      xt = fp8_new(K, M, x);
+      qx.col_codes = xt.codes();
+      qx.col_scales = xt.scales();
+    }
+    launch_fp8_quant(qx, s);
+    launched();
+    auto y = torch::empty({M, O}, x.options().memory_format(c10::MemoryFormat::Contiguous));
+    fp8_product(xq, wt, bias_of(bc, O, x), y);
+    ctx->save_for_backward({wq.mem, xt.mem});
+    ctx->saved_data["M"] = M;
+    ctx->saved_data["K"] = K;
+    ctx->saved_data["O"] = O;
+    ctx->saved_data["wt"] = (int64_t)W.scalar_type();
+    ctx->saved_data["bs"] = b.has_value() ? c10::IValue(b->sizes().vec()) : c10::IValue();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    first_order_only();
+    c10::DeviceGuard guard(g[0].device());
+    auto& sd = ctx->saved_data;
+    const int64_t M = sd["M"].toInt(), K = sd["K"].toInt(), O = sd["O"].toInt();
+    const auto sv = ctx->get_saved_variables();
+    const bool has_b = !sd["bs"].isNone();
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1),
+               want_b = has_b && ctx->needs_input_grad(2);
+    const Tensor dy = rows_of(g[0], M, O);
+    Tensor dx, dW, db, slab;
+    auto f32 = dy.options().dtype(torch::kFloat32);
+    auto q = quant_args(dy, M, O, false);
+    Fp8Buf dq, dt;
+    if (want_x) {
+      dq = fp8_new(M, O, dy);
+      q.row_codes = dq.codes();
+      q.row_scales = dq.scales();
+    }
+    if (want_w) {
+      dt = fp8_new(O, M, dy);
+      q.col_codes = dt.codes();
+      q.col_scales = dt.scales();
+    }
+    if (want_b) {
+      db = M ? torch::empty(sd["bs"].toIntVector(), f32) : torch::zeros(sd["bs"].toIntVector(), f32);
+      slab = torch::empty({(M + 127) / 128, O}, f32);
+      q.colsum = db.data_ptr<float>();
+      q.slab = slab.data_ptr<float>();
+    }
+    if (want_x || want_w || want_b) {
+      launch_fp8_quant(q, stream_of(dy));
+      launched();
+    }
+    if (want_x) {
+      dx = torch::empty({M, K}, dy.options());
+      fp8_product(dq, fp8_buf(sv[0], K, O), nullptr, dx);
+    }
+    if (want_w) {
+      dW = torch::empty({K, O}, dy.options().dtype((at::ScalarType)sd["wt"].toInt()));
+      if (M) fp8_product(fp8_buf(sv[1], K, M), dt, nullptr, dW);
+      else dW.zero_();
+    }
+    return {dx, dW, db, Tensor()};
+  }
+};
+
+Tensor block_fp8_fc(const Tensor& x, const Tensor& W, const OptTensor& b) {
+  BK_CHECK(x.is_cuda() && x.dim() == 2 && W.dim() == 2 && x.size(1) == W.size(0) && x.size(1) > 0 && W.size(1) > 0 &&
+               x.device() == W.device(),
+           "x [N, K] and W [K, O] must be GPU matrices on one device");
+  block_type(x, "x");
+  block_type(W, "W");
+  fp8_dims(x.size(0), x.size(1));
+  fp8_dims(W.size(1), 1);
+  return Fp8FcFn::apply(x, W, b, wants_grad({x, W, b}));
+}
+
 }  // namespace
 
 void bind_block(py::module_& m) {
   m.def("block_dropout", &block_dropout);
   m.def("block_residual", &block_residual);
+  m.def("block_fp8_quantize", &block_fp8_quantize);
+  m.def("block_fp8_matmul", [](const Tensor& a, const Tensor& sa, const Tensor& b, const Tensor& sb, int64_t K,
+                               const OptTensor& bias, py::object dtype) {
+    return block_fp8_matmul(a, sa, b, sb, K, bias, torch::python::detail::py_object_to_dtype(dtype));
+  });
+  m.def("block_fp8_fc_packed", &block_fp8_fc_packed);
+  m.def("block_fp8_fc", &block_fp8_fc);
 }
 
 }  // namespace pbx

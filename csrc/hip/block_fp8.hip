@@ -1,0 +1,537 @@
+// 8-bit fc: e4m3 operands with one power-of-two scale for each block of 128,
+// hand-written for gfx950.
+//
+// Quantisation: a = largest finite |v| of the block, e the least exponent with
+// a <= 448 * 2^e, code = e4m3(v * 2^-e) rounded to the nearest, halves to
+// even.  The scale is a power of two, so v * 2^-e is exact and the code holds
+// the one rounding there is (half a step, 2^-4 of the value); what it costs
+// against a free scale is at most one bit at the small end of the block's
+// range, never precision.  Values that are not finite become NaN codes.
+//
+// Product, results of 16 bits: v_mfma_scale_f32_16x16x128_f8f6f4 takes an
+// exponent byte for each 32 values of either operand; four equal bytes are one
+// block of 128, so the instruction applies the scales with no vector work
+// beside it, and one instruction is exactly one block deep.  Inside the
+// instruction each run of 8 products is aligned to its largest and what lies
+// more than 13 bits below that is dropped (measured; runs are added in full
+// fp32): up to 2^-13 of a run's largest product a value, under the half step
+// of a 16-bit result for all but sums that cancel, and far under the 2^-4 that
+// the codes themselves are rounded by.  That is 4.2 PFLOP/s from registers.
+// Results of 32 bits: the codes become bf16 with their scale in registers
+// (v_cvt_scalef32_pk_bf16_fp8; 4 significant bits fit) and go through
+// v_mfma_f32_16x16x32_bf16, which drops nothing above 2^-23 (2.3 PFLOP/s).
+// A scale holds for all 128 values of its block, so any order of them within
+// the instructions is right as long as both operands use the same.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "block_ops.h"
+
+namespace pbx {
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// ---------------------------------------------------------------- quantisation
+// |v| as an integer that orders like it; 0 where v is not finite
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+// exponent byte of a block whose largest finite |v| has these bits: with
+// |v| = 1.f * 2^(E - 127), the least e such that 1.f * 2^(E-127) <= 1.75 * 2^(8+e)
+__device__ __forceinline__ int scale_byte(uint32_t bits) {
+  const int e = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return e < 0 ? 0 : e;
+}
+// 2^(127 - byte): bytes are 0 .. 247, so this is a normal number
+__device__ __forceinline__ float inverse_scale(int byte) { return __builtin_bit_cast(float, (uint32_t)(254 - byte) << 23); }
+__device__ __forceinline__ float scaled(float v, float inv) {
+  return finite_bits(v) || v == 0.f ? v * inv : __builtin_bit_cast(float, 0x7fc00000u);
+}
+// four codes, the first in the low byte
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+// Blocks along a row only: 16 lanes a block, 8 values a lane.
+template <typename E>
+__global__ __launch_bounds__(256) void k_fp8_quant_rows(Fp8QuantArgs a) {
+  const int64_t nb = fp8_kp(a.K) / 128, sp = fp8_sp(a.K);
+  const int64_t blk = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (blk >= a.M * nb) return;  // the same for the 16 lanes of a block
+  const int lane = threadIdx.x & 15;
+  const int64_t row = blk / nb, kb = blk % nb, col = kb * 128 + lane * 8;
+  const int64_t left = a.K - col;
+  float v[8];
+  load8((const E*)a.x + row * a.ld + (left > 0 ? col : 0), left >= 8 ? 8 : left > 0 ? (int)left : 0, v);
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, finite_bits(v[j]));
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+  const int byte = scale_byte(m);
+  const float inv = inverse_scale(byte);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = scaled(v[j], inv);
+  uint2 c{codes4(v[0], v[1], v[2], v[3]), codes4(v[4], v[5], v[6], v[7])};
+  *reinterpret_cast<uint2*>(a.row_codes + row * nb * 128 + col) = c;
+  if (lane == 0) {
+    uint8_t* s = a.row_scales + row * sp;
+    s[kb] = (uint8_t)byte;
+    if (kb == nb - 1)
+      for (int64_t i = nb; i < sp; ++i) s[i] = 127;
+  }
+}
+
+// One 128 x 128 tile a workgroup, read once: codes in blocks along the rows
+// and, transposed, along the columns, and partial column sums.  Thread t holds
+// columns 4 (t % 32) .. + 3 of rows 16 (t / 32) .. + 15: a row's block is one
+// half-wave, and 16 rows of a column are one 16-byte piece of the transposed
+// codes, put together through LDS so that whole 128-byte lines are written.
+template <typename E>
+__global__ __launch_bounds__(256) void k_fp8_quant_tile(Fp8QuantArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t cols[128 * 128];
+  __shared__ uint32_t red[8][128];
+  __shared__ uint32_t tile_max[4];
+  const int64_t k0 = (int64_t)blockIdx.x * 128, m0 = (int64_t)blockIdx.y * 128;
+  const int t = threadIdx.x, cq = (t & 31) * 4, rq = t >> 5;
+  const int64_t rows = a.M - m0, width = a.K - k0;
+  const int64_t kp = fp8_kp(a.K), ksp = fp8_sp(a.K), mp = fp8_kp(a.M), msp = fp8_sp(a.M);
+  float v[16][4];
+  const int valid = width - cq >= 4 ? 4 : width - cq > 0 ? (int)(width - cq) : 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = rq * 16 + i;
+    const E* p = (const E*)a.x + (m0 + r) * a.ld + k0 + cq;
+    typedef E vec __attribute__((ext_vector_type(4), aligned(sizeof(E))));
+    if (r < rows && valid == 4) {
+      const vec x = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = (float)x[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = r < rows && j < valid ? (float)p[j] : 0.f;
+    }
+  }
+  if (a.slab) {
+    float* fr = reinterpret_cast<float*>(red);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s += v[i][j];
+      fr[rq * 128 + cq + j] = s;
+    }
+    __syncthreads();
+    if (t < 128 && t < width) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) s += fr[w * 128 + t];
+      a.slab[(int64_t)blockIdx.y * a.K + k0 + t] = s;
+    }
+    __syncthreads();
+  }
+  uint32_t rowmax[16], colmax[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t b = finite_bits(v[i][j]);
+      m = max(m, b);
+      colmax[j] = max(colmax[j], b);
+    }
+    rowmax[i] = m;
+  }
+  int tile_byte = 0;
+  if (a.tile) {
+    uint32_t m = max(max(colmax[0], colmax[1]), max(colmax[2], colmax[3]));
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+    if ((t & 63) == 0) tile_max[t >> 6] = m;
+    __syncthreads();
+    tile_byte = scale_byte(max(max(tile_max[0], tile_max[1]), max(tile_max[2], tile_max[3])));
+  }
+  if (a.row_codes) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      uint32_t m = rowmax[i];
+      int byte = tile_byte;
+      if (!a.tile) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+        byte = scale_byte(m);
+      }
+      const int r = rq * 16 + i;
+      if (r >= rows) continue;
+      const float inv = inverse_scale(byte);
+      *reinterpret_cast<uint32_t*>(a.row_codes + (m0 + r) * kp + k0 + cq) =
+          codes4(scaled(v[i][0], inv), scaled(v[i][1], inv), scaled(v[i][2], inv), scaled(v[i][3], inv));
+      if ((t & 31) == 0) {
+        uint8_t* s = a.row_scales + (m0 + r) * ksp;
+        s[blockIdx.x] = (uint8_t)byte;
+        if (blockIdx.x == gridDim.x - 1)
+          for (int64_t q = gridDim.x; q < ksp; ++q) s[q] = 127;
+      }
+    }
+  }
+  if (a.col_codes) {
+    if (!a.tile) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) red[rq][cq + j] = colmax[j];
+      __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      int byte = tile_byte;
+      const int c = cq + j;
+      if (!a.tile) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) m = max(m, red[w][c]);
+        byte = scale_byte(m);
+      }
+      const float inv = inverse_scale(byte);
+      uint32_t q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        q[i] = codes4(scaled(v[4 * i][j], inv), scaled(v[4 * i + 1][j], inv), scaled(v[4 * i + 2][j], inv),
+                      scaled(v[4 * i + 3][j], inv));
+      // 16-byte piece rq of column c, pieces turned by the column so that writes and reads spread over the banks
+      *reinterpret_cast<uint4*>(cols + c * 128 + ((rq ^ (c >> 2)) & 7) * 16) = make_uint4(q[0], q[1], q[2], q[3]);
+      if (rq == 0 && c < width) {
+        uint8_t* s = a.col_scales + (k0 + c) * msp;
+        s[blockIdx.y] = (uint8_t)byte;
+        if (blockIdx.y == gridDim.y - 1)
+          for (int64_t i = gridDim.y; i < msp; ++i) s[i] = 127;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = i * 256 + t, c = p >> 3, w = p & 7;
+      if (c < width)
+        *reinterpret_cast<uint4*>(a.col_codes + (k0 + c) * mp + m0 + w * 16) =
+            *reinterpret_cast<const uint4*>(cols + c * 128 + ((w ^ (c >> 2)) & 7) * 16);
+    }
+  }
+}
+
+// out[c] = sum of the slab rows in order: 64 columns a workgroup, 4 waves share the rows
+__global__ __launch_bounds__(256) void k_fp8_colsum(const float* __restrict__ slab, int64_t rows, int64_t K,
+                                                    float* __restrict__ out) {
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (c < K)
+    for (int64_t r = w; r < rows; r += 4) s += slab[r * K + c];
+  red[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && c < K) out[c] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+}
+
+// ---------------------------------------------------------------- product
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// One block of 128 of a row as the instructions take it, 32 codes a lane.
+// FULL: as bf16 values with the scale in them; else codes and exponent bytes.
+template <bool FULL>
+struct Frag;
+template <>
+struct Frag<false> {
+  i32x8 v;
+  int e;
+  __device__ __forceinline__ Frag() {}
+  __device__ __forceinline__ Frag(i32x4 lo, i32x4 hi, uint32_t byte)
+      : v(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), e((int)(byte * 0x01010101u)) {}
+};
+template <>
+struct Frag<true> {
+  bf16x8 v[4];
+  __device__ __forceinline__ Frag() {}
+  __device__ __forceinline__ Frag(i32x4 lo, i32x4 hi, uint32_t byte) {
+    const float scale = __builtin_bit_cast(float, byte << 23);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const i32x4 src = q < 2 ? lo : hi;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int w = src[(q & 1) * 2 + h];
+        const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false),
+                     b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true);
+        v[q][4 * h] = a[0];
+        v[q][4 * h + 1] = a[1];
+        v[q][4 * h + 2] = b[0];
+        v[q][4 * h + 3] = b[1];
+      }
+    }
+  }
+};
+__device__ __forceinline__ f32x4 mfma_blocks(const Frag<false>& a, const Frag<false>& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, c, 0, 0, 0, a.e, 0, b.e);
+}
+__device__ __forceinline__ f32x4 mfma_blocks(const Frag<true>& a, const Frag<true>& b, f32x4 c) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], c, 0, 0, 0);
+  return c;
+}
+
+template <typename C>
+__device__ __forceinline__ void store4(C* p, int valid, f32x4 v) {
+  typedef C vec __attribute__((ext_vector_type(4), aligned(sizeof(C))));
+  if (valid >= 4) {
+    vec x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = (C)v[j];
+    *reinterpret_cast<vec*>(p) = x;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < valid) p[j] = (C)v[j];
+  }
+}
+__device__ __forceinline__ f32x4 bias4(const float* b, int n, int N) {
+  f32x4 v{0.f, 0.f, 0.f, 0.f};
+  if (b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = n + j < N ? b[n + j] : 0.f;
+  }
+  return v;
+}
+
+// 16-B-per-lane LDS-DMA (lane l lands at lds_byte + 16 l); the wait is the caller's
+__device__ __forceinline__ void glds16(const void* gsrc, unsigned lds_byte) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "v"(gsrc), "s"(lds_byte)
+               : "memory");
+}
+__device__ __forceinline__ unsigned lds_addr(const void* p) {
+  return (unsigned)(uintptr_t)((const __attribute__((address_space(3))) char*)p);
+}
+
+// Output tile of WR x WC waves, each MT x NT instruction tiles.  The matrix
+// instruction's rows are b's (columns of the output), its columns a's: a lane
+// then holds 4 consecutive outputs of one row.  LDS: two buffers of BM + BN
+// rows of 128 bytes, filled by LDS-DMA one block ahead; 16-byte piece p of row
+// r sits at place p ^ (r & 7), so the 16 rows that a fragment read touches
+// spread over the banks (the DMA writes lanes in order, so the turn is made in
+// the global address).
+template <int WR, int WC, int MT, int NT, typename C>
+__global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
+  using F = Frag<std::is_same<C, float>::value>;
+  constexpr int BM = WR * MT * 16, BN = WC * NT * 16, W = WR * WC, ROWS = BM + BN;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][ROWS * 128];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int wr = w / WC, wc = w % WC;
+  const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
+  const int64_t kp = fp8_kp(g.K), sp = fp8_sp(g.K);
+  const int nb = (int)(kp / 128), per = (nb + g.ksplit - 1) / g.ksplit;
+  const int kb0 = blockIdx.z * per, kb1 = min(nb, kb0 + per);
+  constexpr int LOADS = ROWS / 8 / W;  // each fills 8 rows
+  static_assert(ROWS % (8 * W) == 0 && BM % 8 == 0, "whole loads");
+  const uint8_t* src[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int r = (i * W + w) * 8 + (lane >> 3), piece = (lane & 7) ^ (r & 7);
+    // rows past the end read the last one: their outputs are not stored
+    const int64_t row = r < BM ? min(m0 + r, g.M - 1) : min(n0 + r - BM, g.N - 1);
+    src[i] = (r < BM ? g.a : g.b) + row * kp + piece * 16 + (int64_t)kb0 * 128;
+  }
+  auto fill = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      glds16(src[i], __builtin_amdgcn_readfirstlane(lds_addr(&lds[buf][(i * W + w) * 1024])));
+      src[i] += 128;
+    }
+  };
+  const int fr = lane & 15, fg = lane >> 4;
+  const uint8_t *psa[MT], *psb[NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) psa[i] = g.sa + (int64_t)min(m0 + (wr * MT + i) * 16 + fr, g.M - 1) * sp;
+#pragma unroll
+  for (int i = 0; i < NT; ++i) psb[i] = g.sb + (int64_t)min(n0 + (wc * NT + i) * 16 + fr, g.N - 1) * sp;
+  uint32_t sa[MT], sb[NT];
+  f32x4 acc[MT][NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto frag = [&](int buf, int row, uint32_t byte) {
+    const uint8_t* p = &lds[buf][row * 128];
+    return F(*reinterpret_cast<const i32x4*>(p + ((fg ^ (row & 7)) * 16)),
+             *reinterpret_cast<const i32x4*>(p + (((fg + 4) ^ (row & 7)) * 16)), byte);
+  };
+  if (kb0 < kb1) fill(0);
+  for (int kb = kb0; kb < kb1; ++kb) {
+    const int buf = (kb - kb0) & 1;
+    if (kb == kb0 || (kb & 3) == 0) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) sa[i] = *reinterpret_cast<const uint32_t*>(psa[i] + (kb & ~3));
+#pragma unroll
+      for (int i = 0; i < NT; ++i) sb[i] = *reinterpret_cast<const uint32_t*>(psb[i] + (kb & ~3));
+    }
+    // this wave's part of the buffer has arrived; after the barrier everybody's has, and nobody reads the other one
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (kb + 1 < kb1) fill(buf ^ 1);
+    const int sh = (kb & 3) * 8;
+    F fb[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) fb[j] = frag(buf, BM + (wc * NT + j) * 16 + fr, sb[j] >> sh & 0xffu);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const F fa = frag(buf, (wr * MT + i) * 16 + fr, sa[i] >> sh & 0xffu);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = mfma_blocks(fb[j], fa, acc[i][j]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int m = m0 + (wr * MT + i) * 16 + fr;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int n = n0 + (wc * NT + j) * 16 + fg * 4;
+      if (m >= g.M || n >= g.N) continue;
+      if (g.ksplit > 1) {
+        store4(g.slab + ((int64_t)blockIdx.z * g.M + m) * g.N + n, g.N - n, acc[i][j]);
+      } else {
+        store4((C*)g.c + (int64_t)m * g.N + n, g.N - n, acc[i][j] + bias4(g.bias, n, g.N));
+      }
+    }
+  }
+}
+
+// c = sum of the slices in order (+ bias)
+template <typename C>
+__global__ __launch_bounds__(256) void k_fp8_join(Fp8GemmArgs g) {
+  const int64_t n4 = ((int64_t)g.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n4 * g.M) return;
+  const int64_t m = i / n4;
+  const int n = (int)(i % n4) * 4;
+  typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
+  f32x4 s{0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < g.ksplit; ++k) {
+    const float* p = g.slab + ((int64_t)k * g.M + m) * g.N + n;
+    if (n + 4 <= g.N) {
+      s += *reinterpret_cast<const vec*>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n + j < g.N) s[j] += p[j];
+    }
+  }
+  store4((C*)g.c + m * g.N + n, g.N - n, s + bias4(g.bias, n, g.N));
+}
+
+// Up to 16 MT rows of a: the bytes of b are the cost, so no LDS staging.  A
+// workgroup takes 16 rows of b, its 8 waves share the blocks of K and join
+// their sums through LDS in order.
+template <int MT, typename C>
+__global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
+  __shared__ f32x4 part[8][MT][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 15, fg = lane >> 4;
+  const int64_t kp = fp8_kp(g.K), sp = fp8_sp(g.K);
+  const int nb = (int)(kp / 128);
+  const int n0 = blockIdx.x * 16;
+  const int64_t brow = min(n0 + fr, g.N - 1);
+  const uint8_t* pb = g.b + brow * kp + fg * 32;
+  const uint8_t* psb = g.sb + brow * sp;
+  const uint8_t *pa[MT], *psa[MT];
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int64_t r = min(i * 16 + fr, g.M - 1);
+    pa[i] = g.a + r * kp + fg * 32;
+    psa[i] = g.sa + r * sp;
+    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  using F = Frag<std::is_same<C, float>::value>;
+  auto load = [](const uint8_t* p, uint32_t byte) {
+    return F(*reinterpret_cast<const i32x4*>(p), *reinterpret_cast<const i32x4*>(p + 16), byte);
+  };
+  for (int kb = w; kb < nb; kb += 8) {
+    const F fb = load(pb + (int64_t)kb * 128, psb[kb]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = mfma_blocks(fb, load(pa[i] + (int64_t)kb * 128, psa[i][kb]), acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) part[w][i][lane] = acc[i];
+  __syncthreads();
+  if (w < MT) {
+    f32x4 s = part[0][w][lane];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += part[k][w][lane];
+    const int m = w * 16 + fr, n = n0 + fg * 4;
+    if (m < g.M && n < g.N) store4((C*)g.c + (int64_t)m * g.N + n, g.N - n, s + bias4(g.bias, n, g.N));
+  }
+}
+
+template <typename C>
+void gemm(const Fp8GemmArgs& g, hipStream_t s) {
+  if (g.M <= 64) {
+    const dim3 grid((g.N + 15) / 16);
+    if (g.M <= 16) hipLaunchKernelGGL((k_fp8_skinny<1, C>), grid, dim3(512), 0, s, g);
+    else if (g.M <= 32) hipLaunchKernelGGL((k_fp8_skinny<2, C>), grid, dim3(512), 0, s, g);
+    else hipLaunchKernelGGL((k_fp8_skinny<4, C>), grid, dim3(512), 0, s, g);
+    return;
+  }
+  const dim3 grid((g.N + 127) / 128, (g.M + 127) / 128, g.ksplit);
+  hipLaunchKernelGGL((k_fp8_gemm<2, 2, 4, 4, C>), grid, dim3(256), 0, s, g);
+  if (g.ksplit > 1) {
+    const int64_t n = ((int64_t)g.N + 3) / 4 * g.M;
+    hipLaunchKernelGGL(k_fp8_join<C>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, g);
+  }
+}
+
+}  // namespace
+
+int fp8_gemm_ksplit(int M, int N, int64_t K) {
+  if (M <= 64) return 1;
+  const int64_t tiles = (int64_t)((M + 127) / 128) * ((N + 127) / 128), nb = fp8_kp(K) / 128;
+  // about one workgroup a CU, at least 4 blocks of K each
+  int64_t split = 256 / tiles;
+  if (split > nb / 4) split = nb / 4;
+  if (split < 1) split = 1;
+  const int64_t per = (nb + split - 1) / split;
+  return (int)((nb + per - 1) / per);  // no empty slice
+}
+
+void launch_fp8_gemm(const Fp8GemmArgs& g, hipStream_t s) {
+  if (g.M == 0 || g.N == 0) return;
+  if (g.ct == kF32) gemm<float>(g, s);
+  else if (g.ct == kBF16) gemm<__bf16>(g, s);
+  else gemm<_Float16>(g, s);
+}
+
+namespace {
+template <typename E>
+void quant(const Fp8QuantArgs& a, hipStream_t s) {
+  const int64_t kb = fp8_kp(a.K) / 128;
+  if (!a.col_codes && !a.colsum && !a.tile) {
+    hipLaunchKernelGGL(k_fp8_quant_rows<E>, dim3((unsigned)((a.M * kb + 15) / 16)), dim3(256), 0, s, a);
+    return;
+  }
+  const int64_t mb = (a.M + 127) / 128;
+  hipLaunchKernelGGL(k_fp8_quant_tile<E>, dim3((unsigned)kb, (unsigned)mb), dim3(256), 0, s, a);
+  if (a.colsum)
+    hipLaunchKernelGGL(k_fp8_colsum, dim3((unsigned)((a.K + 63) / 64)), dim3(256), 0, s, a.slab, mb, a.K, a.colsum);
+}
+}  // namespace
+
+void launch_fp8_quant(const Fp8QuantArgs& a, hipStream_t s) {
+  if (a.M == 0 || a.K == 0) return;
+  if (a.t == kF32) quant<float>(a, s);
+  else if (a.t == kBF16) quant<__bf16>(a, s);
+  else quant<_Float16>(a, s);
+}
+
+}  // namespace pbx

@@ -6,6 +6,8 @@
 
 #include <cstdint>
 
+#define PBX_FP8_HD __host__ __device__ inline
+
 namespace pbx {
 
 // element types of the dense-block operators
@@ -68,6 +70,40 @@ int residual_slab_rows(int64_t M, int D);
 constexpr int kResidualMaxD = 16384;
 void launch_residual_fwd(const ResidualArgs& a, hipStream_t s);
 void launch_residual_bwd(const ResidualArgs& a, hipStream_t s);
+
+// ---------------------------------------------------------------- 8-bit blocks
+// A matrix [rows, K] held in e4m3 with one power-of-two scale for each block
+// of 128 along K: codes [rows][Kp], Kp = K up to a multiple of 128 (padding
+// zero), exponent bytes [rows][Sp], Sp = Kp / 128 up to a multiple of 4; byte
+// e stands for 2^(e - 127).  A block scaled over 128 rows as well repeats its
+// byte in each of them.
+PBX_FP8_HD int64_t fp8_kp(int64_t K) { return (K + 127) / 128 * 128; }
+PBX_FP8_HD int64_t fp8_sp(int64_t K) { return (fp8_kp(K) / 128 + 3) / 4 * 4; }
+
+struct Fp8QuantArgs {
+  const void* x = nullptr;  // [M, K], row stride ld
+  BlockType t = kF32;
+  int64_t M = 0, K = 0, ld = 0;
+  int tile = 0;  // one scale for 128 x 128, both outputs alike
+  uint8_t *row_codes = nullptr, *row_scales = nullptr;  // x in blocks along K: [M][fp8_kp(K)], [M][fp8_sp(K)]
+  uint8_t *col_codes = nullptr, *col_scales = nullptr;  // x^T in blocks along M: [K][fp8_kp(M)], [K][fp8_sp(M)]
+  float* colsum = nullptr;                              // [K] fp32 column sums of x
+  float* slab = nullptr;                                // [ceil(M / 128)][K] for them
+};
+void launch_fp8_quant(const Fp8QuantArgs& a, hipStream_t s);
+
+struct Fp8GemmArgs {  // c [M, N] = a [M, K] b [N, K]^T (+ bias [N])
+  const uint8_t *a = nullptr, *b = nullptr, *sa = nullptr, *sb = nullptr;
+  int M = 0, N = 0;
+  int64_t K = 0;  // logical: strides are fp8_kp(K), fp8_sp(K)
+  const float* bias = nullptr;
+  void* c = nullptr;
+  BlockType ct = kF32;
+  int ksplit = 1;         // slices of K; more than one goes through the slab
+  float* slab = nullptr;  // [ksplit][M][N]
+};
+int fp8_gemm_ksplit(int M, int N, int64_t K);
+void launch_fp8_gemm(const Fp8GemmArgs& a, hipStream_t s);
 
 #ifdef __HIPCC__
 // ---------------------------------------------------------------- device helpers

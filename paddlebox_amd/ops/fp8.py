@@ -1,0 +1,207 @@
+"""fc in 8-bit floating point with a scale for each block of 128: the block-scaled
+member of the scaled_fc family (``ops/ctr_ext.py``: scaled_fc, scaled_int8fc).
+
+A block of values (128 along the reduction axis, or 128 x 128 of a weight) is
+held as e4m3 codes and one exponent byte e, which stands for the scale
+2^(e - 127): the least power of two, no less than 2^-127, with which the
+block's largest finite value is at most 448.  ``code = e4m3(v / scale)``,
+rounded to the nearest, halves to even; values that are not finite become NaN.
+A power of two divides exactly, so there is one rounding, of half a step
+(2^-4 of the value).
+
+GPU tensors run ``csrc/hip/block_fp8.hip``; the torch expressions here are the
+CPU path and the reference the GPU tests compare against.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Union
+
+import torch
+
+from .. import _native
+
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+BLOCK = 128
+MAX_DIM = 65535 * 128
+
+
+def _padded(k: int) -> int:
+    return (k + BLOCK - 1) // BLOCK * BLOCK
+
+
+@dataclass(frozen=True)
+class Fp8Blocks:
+    """A [rows, cols] matrix in blocks of 128 along its columns.
+
+    ``codes``: float8_e4m3fn [rows, cols up to a multiple of 128], the padding
+    zero.  ``scales``: uint8 [rows, blocks up to a multiple of 4], the exponent
+    byte of each block of each row (a 128 x 128 block repeats its byte in its
+    rows); the padding's value does not matter.  Both contiguous.
+    """
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    cols: int
+
+    def __post_init__(self):
+        c, s = self.codes, self.scales
+        kp = _padded(self.cols)
+        if self.cols < 1 or c.dtype != torch.float8_e4m3fn or c.dim() != 2 or c.shape[1] != kp or not c.is_contiguous():
+            raise ValueError(f"Fp8Blocks: codes must be a contiguous float8_e4m3fn [rows, {kp}] for {self.cols} columns, "
+                             f"not {c.dtype} {list(c.shape)}")
+        sp = (kp // BLOCK + 3) // 4 * 4
+        if s.dtype != torch.uint8 or s.shape != (c.shape[0], sp) or not s.is_contiguous() or s.device != c.device:
+            raise ValueError(f"Fp8Blocks: scales must be a contiguous uint8 [{c.shape[0]}, {sp}] beside the codes, "
+                             f"not {s.dtype} {list(s.shape)} on {s.device}")
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    def dequantize(self) -> torch.Tensor:
+        """The values it stands for, float32 [rows, cols]."""
+        e = self.scales[:, : self.codes.shape[1] // BLOCK].to(torch.int32)
+        v = self.codes.float().reshape(self.rows, e.shape[1], BLOCK) * _two_to(e).unsqueeze(2)
+        return v.reshape(self.codes.shape)[:, : self.cols]
+
+
+def _two_to(byte: torch.Tensor) -> torch.Tensor:
+    """2^(byte - 127) exactly; byte 255 is NaN (as the matrix instruction has it)."""
+    bits = torch.where(byte > 0, byte << 23, torch.full_like(byte, 1 << 22))
+    return torch.where(byte < 255, bits, torch.full_like(byte, 0x7FC00000)).to(torch.int32).view(torch.float32)
+
+
+def _quantize_cpu(x: torch.Tensor, tile: bool) -> Fp8Blocks:
+    m, k = x.shape
+    v = torch.nn.functional.pad(x.float(), (0, -k % BLOCK, 0, -m % BLOCK if tile else 0))
+    a = torch.where(torch.isfinite(v), v.abs(), 0.0).reshape(v.shape[0], v.shape[1] // BLOCK, BLOCK).amax(2)
+    if tile and m:
+        a = a.reshape(-1, BLOCK, a.shape[1]).amax(1).repeat_interleave(BLOCK, 0)
+    f, n = torch.frexp(a)  # a = f 2^n, f in [0.5, 1); 448 = 0.875 * 2^9
+    byte = (n - 9 + (f > 0.875).to(n.dtype) + 127).clamp(min=0) * (a > 0)
+    w = v * _two_to(254 - byte).repeat_interleave(BLOCK, 1)
+    codes = torch.where(torch.isfinite(w), w, float("nan")).to(torch.float8_e4m3fn)[:m].contiguous()
+    scales = torch.nn.functional.pad(byte[:m].to(torch.uint8), (0, -byte.shape[1] % 4), value=127)
+    return Fp8Blocks(codes, scales.contiguous(), k)
+
+
+def _check_matrix(name: str, x: torch.Tensor, who: str):
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"{who}: {name} must be a matrix with at least one column, not {list(x.shape)}")
+    if x.dtype not in _TYPES:
+        raise TypeError(f"{who}: {name} must be float32, bfloat16 or float16, not {x.dtype}")
+    if max(x.shape) > MAX_DIM:
+        raise ValueError(f"{who}: {name} has more than {MAX_DIM} rows or columns")
+
+
+def fp8_quantize(x: torch.Tensor, block: str = "row", transposed: bool = False) -> Fp8Blocks:
+    """x [M, K] in 8-bit blocks.
+
+    ``block``: "row", a scale for each 128 values along the reduction axis
+    (activations, gradients), or "tile", a scale for each 128 x 128 (weights:
+    x and x^T then hold the same values).
+    ``transposed``: the blocks of x^T [K, M], reduction along x's rows -- the
+    form ``fp8_matmul`` and ``scaled_fp8fc`` take a weight W [K, O] in is
+    ``fp8_quantize(W, "tile", transposed=True)``.
+    """
+    _check_matrix("x", x, "fp8_quantize")
+    if block not in ("row", "tile"):
+        raise ValueError(f"fp8_quantize: block must be 'row' or 'tile', not {block!r}")
+    if transposed and x.shape[0] < 1:
+        raise ValueError("fp8_quantize: no rows to reduce over")
+    if x.is_cuda:
+        codes, scales = _native.hip().block_fp8_quantize(x, block == "tile", transposed)
+        return Fp8Blocks(codes, scales, x.shape[0] if transposed else x.shape[1])
+    return _quantize_cpu(x.detach().t() if transposed else x.detach(), block == "tile")
+
+
+def _check_bias(b: Optional[torch.Tensor], n: int, device, who: str):
+    if b is not None and (b.dtype != torch.float32 or b.numel() != n or b.device != device):
+        raise ValueError(f"{who}: the bias must be float32 with {n} values on {device}, "
+                         f"not {b.dtype} {list(b.shape)} on {b.device}")
+
+
+def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None,
+               out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """a [M, K] times b [N, K] transposed (+ bias [N], float32), accumulated in
+    32 bits and rounded once to ``out_dtype``.  Not differentiable.
+
+    On the GPU a 16-bit result comes from the 8-bit matrix instructions, which
+    drop, of each run of 8 products along K, what lies more than 13 bits under
+    the run's largest; a float32 result comes from bf16 instructions at half
+    their rate, which do not (held values under 2^-126 count as zero there).
+    """
+    if a.cols != b.cols:
+        raise ValueError(f"fp8_matmul: a has {a.cols} columns, b {b.cols}")
+    if a.codes.device != b.codes.device:
+        raise ValueError(f"fp8_matmul: a is on {a.codes.device}, b on {b.codes.device}")
+    if out_dtype not in _TYPES:
+        raise TypeError(f"fp8_matmul: the result is float32, bfloat16 or float16, not {out_dtype}")
+    if max(a.rows, b.rows, a.cols) > MAX_DIM:
+        raise ValueError(f"fp8_matmul: more than {MAX_DIM} rows or columns")
+    _check_bias(bias, b.rows, a.codes.device, "fp8_matmul")
+    if a.codes.is_cuda:
+        return _native.hip().block_fp8_matmul(a.codes, a.scales, b.codes, b.scales, a.cols, bias, out_dtype)
+    y = a.dequantize() @ b.dequantize().t()
+    return (y + bias.detach().reshape(1, -1) if bias is not None else y).to(out_dtype)
+
+
+class _Fp8FcCpu(torch.autograd.Function):
+    """The arithmetic of block_fp8.hip in torch."""
+
+    @staticmethod
+    def forward(ctx, x, W, b):
+        wq = fp8_quantize(W, "tile").dequantize()
+        ctx.save_for_backward(x, wq)
+        ctx.wdtype, ctx.bshape = W.dtype, b.shape if b is not None else None
+        y = fp8_quantize(x).dequantize() @ wq
+        return (y + b.reshape(1, -1) if b is not None else y).to(x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, wq = ctx.saved_tensors
+        dx = (fp8_quantize(dy).dequantize() @ wq.t()).to(x.dtype)
+        if x.shape[0]:
+            dW = fp8_quantize(x, transposed=True).dequantize() @ fp8_quantize(dy, transposed=True).dequantize().t()
+        else:
+            dW = torch.zeros_like(wq)
+        return dx, dW.to(ctx.wdtype), (dy.float().sum(0).reshape(ctx.bshape) if ctx.bshape is not None else None)
+
+
+def scaled_fp8fc(x: torch.Tensor, W: Union[torch.Tensor, Fp8Blocks], b: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """fc with 8-bit operands: y = q(x) q(W) + b, accumulated in 32 bits and
+    rounded once to x's type.
+
+    x [N, K] and W [K, O]: float32, bfloat16 or float16; b: float32 with O
+    values, or None.  x is held in blocks of 128 along K, W in 128 x 128
+    blocks.  Differentiable once: dx = q(dy) q(W)^T with dy in blocks along O,
+    dW = q(x)^T q(dy) with both in blocks of 128 rows of the batch (straight
+    through the rounding), db = column sums of dy; dx has x's type, dW W's.
+    ``W`` may be packed, ``fp8_quantize(W, "tile", transposed=True)``, for
+    serving: then nothing is differentiable.
+    """
+    _check_matrix("x", x, "scaled_fp8fc")
+    packed = isinstance(W, Fp8Blocks)
+    if packed:
+        if W.cols != x.shape[1]:
+            raise ValueError(f"scaled_fp8fc: x has {x.shape[1]} columns, the packed weight {W.cols}")
+        device, n = W.codes.device, W.rows
+        if torch.is_grad_enabled() and (x.requires_grad or b is not None and b.requires_grad):
+            raise ValueError("scaled_fp8fc: a packed weight is for inference; detach x and b or use torch.no_grad()")
+    else:
+        _check_matrix("W", W, "scaled_fp8fc")
+        if W.shape[0] != x.shape[1]:
+            raise ValueError(f"scaled_fp8fc: x {list(x.shape)} and W {list(W.shape)} do not fit")
+        device, n = W.device, W.shape[1]
+    if device != x.device:
+        raise ValueError(f"scaled_fp8fc: x is on {x.device}, the weight on {device}")
+    _check_bias(b, n, x.device, "scaled_fp8fc")
+    if x.is_cuda:
+        if packed:
+            return _native.hip().block_fp8_fc_packed(x, W.codes, W.scales, b)
+        return _native.hip().block_fp8_fc(x, W, b)
+    if packed:
+        return fp8_matmul(fp8_quantize(x), W, b, out_dtype=x.dtype)
+    return _Fp8FcCpu.apply(x, W, b)

@@ -122,10 +122,61 @@ class Residual:
 
 
 def near(got, want, mag, roundings=Residual.ROUNDINGS):
-    """Asserts |got - want| <= half a step of got's type (twice: the value and its neighbour's step) + roundings * mag."""
-    got64 = got.detach().double().cpu()
-    tiny = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps  # half a subnormal step and more
-    lim = HALF[got.dtype] * want.abs() * (1 + 2 * HALF[got.dtype]) + roundings * mag * (1 + HALF[got.dtype]) + tiny
-    bad = ~((got64 - want).abs() <= lim)
+    """Asserts |got - want| <= half a step of got's type + roundings * mag; where that reaches past the type's largest
+    value, infinity is right too."""
+    got64, f = got.detach().double().cpu(), torch.finfo(got.dtype)
+    half_subnormal = f.smallest_normal * f.eps / 2
+    lim = HALF[got.dtype] * want.abs() + roundings * mag * (1 + HALF[got.dtype]) + half_subnormal
+    over = (got64 == torch.sign(want) * float("inf")) & (want.abs() + lim > f.max)
+    bad = ~(((got64 - want).abs() <= lim) | over)
     assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} values off, worst "
                            f"{float(((got64 - want).abs() / lim).nan_to_num(1e30).max()):.3g} x the bound")
+
+
+# ------------------------------------------------------------------ 8-bit blocks
+def held(x, rows, cols):
+    """x (any float type) as blocks of rows x cols hold it in e4m3 with a power-of-two scale, in 64 bits, from the
+    format's definition: three mantissa bits, least exponent -6, largest value 448, halves to even; the scale is the
+    least 2^e, e >= -127, with which the block's largest finite value is at most 448."""
+    x = x.detach().double().cpu()
+    m, k = x.shape
+    p = x.new_zeros(m + -m % rows, k + -k % cols)
+    p[:m, :k] = x
+    v = p.view(p.shape[0] // rows, rows, p.shape[1] // cols, cols)
+    big = torch.where(torch.isfinite(v), v.abs(), 0.0).amax(dim=(1, 3), keepdim=True) if v.numel() else v.new_zeros(
+        v.shape[0], 1, v.shape[2], 1)
+    f, n = torch.frexp(big / 448)  # big / 448 may be rounded: 2^e * 448 is compared exactly below
+    e = n.double()
+    e = torch.where(big <= 448 * 2.0 ** (e - 1), e - 1, e)
+    e = torch.where(big > 448 * 2.0 ** e, e + 1, e).clamp(min=-127)
+    v = v / 2.0 ** e
+    _, n = torch.frexp(v)  # |v| in [2^(n-1), 2^n)
+    step = 2.0 ** ((n.double() - 1).clamp(min=-6) - 3)
+    out = torch.round(v / step) * step * 2.0 ** e
+    return torch.where(torch.isfinite(v), out, float("nan")).view(p.shape)[:m, :k]
+
+
+def product_near(got, a, b, bias=None, exact_runs=True):
+    """got = a b^T (+ bias), a [M, K] and b [N, K] the held values (64 bits).  Products of e4m3 values are exact in 32
+    bits, so a sum is off by at most one rounding (2^-24 of the terms so far) an addition -- K of them, a few for slices
+    and the bias -- and half a step of got's type.  With exact_runs=False (the GPU) a 16-bit result may lose, of each
+    product, what lies below 2^-13 of the largest in its run of 8, and a 32-bit result a subnormal operand: the held
+    values become bf16 operands, whose least normal value is 2^-126, so up to the value itself times the other operand."""
+    want = a @ b.t()
+    mag = a.abs() @ b.abs().t()
+    lost = 0.0
+    if not exact_runs and got.dtype == torch.float32:
+        asub, bsub = (torch.where(t.abs() < 2.0 ** -126, t.abs(), 0.0) for t in (a, b))
+        lost = asub @ b.abs().t() + a.abs() @ bsub.t()
+    if not exact_runs and got.dtype != torch.float32:
+        pad = torch.nn.functional.pad
+        k = a.shape[1]
+        ar, br = (pad(t.abs(), (0, -k % 8)).reshape(t.shape[0], -1, 8) for t in (a, b))
+        for i in range(ar.shape[1]):
+            lost = lost + (ar[:, None, i] * br[None, :, i]).amax(2)
+        lost = lost * 8 * 2.0 ** -13
+    if bias is not None:
+        want = want + bias.detach().double().cpu()
+        mag = mag + bias.detach().double().cpu().abs()
+    r = (a.shape[1] + 64) * 2.0 ** -24
+    near(got, want, mag + lost / r, roundings=r)
