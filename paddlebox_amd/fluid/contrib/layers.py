@@ -6,9 +6,13 @@ fused_seqpool_cvm :1750, ..._with_diff_thres :1833, ..._with_conv :1912,
 ..._with_pcoc :1979, ..._tradew :2049, ..._with_credit :2107,
 cross_norm_layer_hadamard :2163, scaled_fc :2587, scaled_int8fc :2648,
 fused_seqpool_concat :2726, fused_concat :2795, fused_seq_tensor :2834).
+scaled_fp8fc, fused_residual_norm and counter_dropout have no counterpart
+there: the dense blocks of a deep tower.
 Kernels: ``paddlebox_amd/fluid/kernels.py`` -> ``paddlebox_amd/ops``.
 """
 from __future__ import annotations
+
+import zlib
 
 import numpy as np
 
@@ -219,6 +223,89 @@ def scaled_int8fc(input, param_size, param_attr, bias_size, bias_attr, input_sca
                       "weight_expand_factor": float(weight_expand_factor),
                       "weight_clip_factor": float(weight_clip_factor), "int8_range": float(int8_range)})
     return helper.append_activation(out, act)
+
+
+def scaled_fp8fc(input, param_size, param_attr, bias_size, bias_attr, act=None):  # noqa: A002
+    """fc with operands in 8-bit floating point, a power-of-two scale for each
+    block of 128 (``ops.fp8.scaled_fp8fc``): the member of the scaled_fc family
+    that needs no hand-set factors.  ``param_size`` [in, out]; ``bias_attr``
+    False: no bias."""
+    helper = LayerHelper("scaled_fp8fc")
+    w = helper.create_parameter(param_attr, list(param_size), input.dtype)
+    b = helper.create_parameter(bias_attr, list(bias_size), input.dtype)
+    out = helper.create_variable_for_type_inference(input.dtype, (-1, param_size[1]))
+    helper.append_op("scaled_fp8fc", {"Input": [input], "W": [w], "Bias": [b] if b is not None else []}, {"Out": [out]})
+    return helper.append_activation(out, act)
+
+
+def _mask_state(helper, seed):
+    """The persistable (seed, step) a layer's dropout mask is drawn from: the
+    step counts the layer's training batches, so a resumed run goes on with
+    the masks of an uninterrupted one.  Without a seed, each layer takes its
+    own from its name."""
+    if seed is None:
+        seed = zlib.crc32(helper.name.encode())
+    v = helper.block.create_var(f"{helper.name}.mask_state", [2], "int64", persistable=True, stop_gradient=True)
+    sb = helper.startup_program.global_block()
+    if not sb.has_var(v.name):
+        sv = sb.create_var(v.name, [2], "int64", persistable=True)
+        sb.append_op("init_param", outputs={"Out": [sv]},
+                     attrs={"initializer": I.NumpyArrayInitializer(np.array([int(seed), 0], dtype=np.int64))})
+    return v
+
+
+def counter_dropout(x, dropout_prob, is_test=False, seed=None, name=None,
+                    dropout_implementation="downgrade_in_infer"):
+    """``fluid.layers.dropout`` with the mask a function of (seed, training
+    step, element), drawn again in the backward and never stored
+    (``ops.dropout.dropout``)."""
+    helper = LayerHelper("counter_dropout", name)
+    out = helper.create_variable_for_type_inference(x.dtype, x.shape, x.lod_level)
+    helper.append_op("counter_dropout", {"X": [x], "MaskState": [_mask_state(helper, seed)]}, {"Out": [out]},
+                     {"dropout_prob": float(dropout_prob), "is_test": is_test,
+                      "dropout_implementation": dropout_implementation})
+    return out
+
+
+def fused_residual_norm(input, branch, x_scale=1.0, y_scale=1.0, gate=None, gate_act="none", post_norm="none",  # noqa: A002
+                        pre_norm="rms", epsilon=1e-6, dropout_prob=0.0, is_test=False, seed=None, name=None):
+    """The residual stream after a block, and the next block's input
+    (``ops.residual.residual_norm``):
+
+        r = x_scale * input + y_scale * gate * drop(post_norm(branch)),   h = pre_norm(r)
+
+    ``post_norm`` / ``pre_norm``: "none", "rms" or "layer", with weights (and
+    biases) of their own.  ``gate``: None, "channel" (a parameter for each
+    column, starting at 1), or a variable [-1, 1] or of branch's shape.
+    Returns (r, h); h is None without a pre_norm."""
+    helper = LayerHelper("fused_residual_norm", name)
+    D = int(branch.shape[-1])
+    ins = {"X": [input], "Y": [branch]}
+
+    def param(key, suffix, value):
+        ins[key] = [helper.create_parameter(ParamAttr(name=f"{helper.name}.{suffix}", initializer=I.Constant(value)), [D],
+                                            "float32")]
+
+    for kind, key in ((post_norm, "post"), (pre_norm, "pre")):
+        if kind not in ("none", "rms", "layer"):
+            raise ValueError(f"fused_residual_norm: {key}_norm must be 'none', 'rms' or 'layer', not {kind!r}")
+        if kind != "none":
+            param(f"{key}_weight", f"{key}_w", 1.0)
+        if kind == "layer":
+            param(f"{key}_bias", f"{key}_b", 0.0)
+    if gate == "channel":
+        param("gate", "gate", 1.0)
+    elif gate is not None:
+        ins["gate"] = [gate]
+    if dropout_prob:
+        ins["MaskState"] = [_mask_state(helper, seed)]
+    r = helper.create_variable_for_type_inference(input.dtype, input.shape)
+    h = helper.create_variable_for_type_inference(branch.dtype, branch.shape) if pre_norm != "none" else None
+    helper.append_op("fused_residual_norm", ins, {"R": [r], "H": [h] if h is not None else []},
+                     {"x_scale": float(x_scale), "y_scale": float(y_scale), "gate_act": gate_act, "post_norm": post_norm,
+                      "pre_norm": pre_norm, "epsilon": float(epsilon), "dropout_prob": float(dropout_prob),
+                      "is_test": is_test})
+    return r, h
 
 
 def fused_seqpool_concat(input, offsets=None, dims=None):  # noqa: A002

@@ -20,6 +20,9 @@ import torch.nn.functional as F
 
 from ..ops import ctr as ctr_ops
 from ..ops import ctr_ext
+from ..ops import dropout as dropout_ops
+from ..ops import fp8 as fp8_ops
+from ..ops import residual as residual_ops
 from ..ops import sparse as sparse_ops
 from ..ps.sparse_engine import SeqpoolParams
 from .framework import torch_dtype
@@ -666,6 +669,56 @@ def k_scaled_int8fc(ctx, op):
     a = op.attrs
     ctx.set(op.outputs["Out"][0], ctr_ext.scaled_int8fc(x, ctx.param(op.inputs["W"][0]),
                                                         ctx.param(op.inputs["Bias"][0]), a))
+
+
+@kernel("scaled_fp8fc")
+def k_scaled_fp8fc(ctx, op):
+    x = _val(ctx.get(op.inputs["Input"][0])).float()
+    b = op.inputs.get("Bias")
+    ctx.set(op.outputs["Out"][0], fp8_ops.scaled_fp8fc(x, ctx.param(op.inputs["W"][0]),
+                                                       ctx.param(b[0]).reshape(-1) if b else None))
+
+
+def _mask_state(ctx, op, device):
+    """The layer's (seed, step) on the step's device."""
+    name = op.inputs["MaskState"][0].name
+    st = ctx.scope.get(name)
+    if st.device != device:  # loaded from a file before the first step
+        st = st.to(device)
+        ctx.scope.set(name, st)
+    return st
+
+
+@kernel("counter_dropout")
+def k_counter_dropout(ctx, op):
+    x = ctx.get(op.inputs["X"][0])
+    v = _val(x)
+    v = v if v.dtype in (torch.float32, torch.bfloat16, torch.float16) else v.float()
+    train = ctx.training and not op.attrs.get("is_test")
+    st = _mask_state(ctx, op, v.device) if train else None
+    y = dropout_ops.dropout(v, op.attrs["dropout_prob"], st, training=train,
+                            mode=op.attrs["dropout_implementation"])
+    if train:
+        st[1:] += 1  # the backward has the values that this forward read
+    ctx.set(op.outputs["Out"][0], Ragged(y, x.offsets, x.B, x.slot) if isinstance(x, Ragged) else y)
+
+
+@kernel("fused_residual_norm")
+def k_fused_residual_norm(ctx, op):
+    a = op.attrs
+    x, y = (_val(ctx.get(op.inputs[k][0])).float() for k in ("X", "Y"))
+    par = {k: ctx.param(op.inputs[k][0]) for k in ("post_weight", "post_bias", "pre_weight", "pre_bias") if op.inputs.get(k)}
+    gate = _val(ctx.get(op.inputs["gate"][0])).float() if op.inputs.get("gate") else None
+    drop = a["dropout_prob"] > 0 and ctx.training and not a.get("is_test")
+    st = _mask_state(ctx, op, x.device) if drop else None
+    r, h = residual_ops.residual_norm(x, y, x_scale=a["x_scale"], y_scale=a["y_scale"], gate=gate,
+                                      gate_act=a["gate_act"], post=a["post_norm"], pre=a["pre_norm"], eps=a["epsilon"],
+                                      p=a["dropout_prob"] if drop else 0.0, seed=st, **par)
+    if drop:
+        st[1:] += 1
+    ctx.set(op.outputs["R"][0], r)
+    if h is not None:
+        ctx.set(op.outputs["H"][0], h)
 
 
 @kernel("fused_concat")

@@ -46,6 +46,7 @@ GRAPH_SAFE_OPS = {
     "__pull_seqpool_cvm", "__fused_mlp", "__ctr_tower", "__cvm_show_click", "data_norm", "concat", "cast", "fill_constant_batch_size_like",
     "sigmoid", "sigmoid_cross_entropy_with_logits", "reduce_mean", "relu", "fc", "elementwise_add",
     "elementwise_mul", "elementwise_sub", "scale", "log_loss", "mean", "reduce_sum", "tanh", "softmax",
+    "scaled_fp8fc", "fused_residual_norm", "counter_dropout",
 }
 
 # transpiler-inserted dense-sync ops (run after backward / after the update):
