@@ -34,6 +34,7 @@ namespace {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // ---------------------------------------------------------------- quantisation
 // |v| as an integer that orders like it; 0 where v is not finite
@@ -240,30 +241,28 @@ __global__ __launch_bounds__(256) void k_fp8_colsum(const float* __restrict__ sl
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-// One block of 128 of a row as the instructions take it, 32 codes a lane.
-// FULL: as bf16 values with the scale in them; else codes and exponent bytes.
+// 32 codes of a row, as the instructions take them from a lane.  FULL: as
+// bf16 values with the scale in them; else codes and the exponent byte.
 template <bool FULL>
 struct Frag;
 template <>
 struct Frag<false> {
   i32x8 v;
-  int e;
+  int e;  // the byte is the low one
   __device__ __forceinline__ Frag() {}
-  __device__ __forceinline__ Frag(i32x4 lo, i32x4 hi, uint32_t byte)
-      : v(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7)), e((int)(byte * 0x01010101u)) {}
+  __device__ __forceinline__ Frag(i32x8 codes, uint32_t byte) : v(codes), e((int)byte) {}
 };
 template <>
 struct Frag<true> {
   bf16x8 v[4];
   __device__ __forceinline__ Frag() {}
-  __device__ __forceinline__ Frag(i32x4 lo, i32x4 hi, uint32_t byte) {
+  __device__ __forceinline__ Frag(i32x8 codes, uint32_t byte) {
     const float scale = __builtin_bit_cast(float, byte << 23);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const i32x4 src = q < 2 ? lo : hi;
+    for (int q = 0; q < 4; ++q)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int w = src[(q & 1) * 2 + h];
+        const int w = codes[q * 2 + h];
         const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false),
                      b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true);
         v[q][4 * h] = a[0];
@@ -271,9 +270,9 @@ struct Frag<true> {
         v[q][4 * h + 2] = b[0];
         v[q][4 * h + 3] = b[1];
       }
-    }
   }
 };
+// 16 x 16 outputs, 128 deep
 __device__ __forceinline__ f32x4 mfma_blocks(const Frag<false>& a, const Frag<false>& b, f32x4 c) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, c, 0, 0, 0, a.e, 0, b.e);
 }
@@ -281,6 +280,19 @@ __device__ __forceinline__ f32x4 mfma_blocks(const Frag<true>& a, const Frag<tru
 #pragma unroll
   for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], c, 0, 0, 0);
   return c;
+}
+// 32 x 32 outputs, 64 deep
+__device__ __forceinline__ f32x16 mfma_blocks(const Frag<false>& a, const Frag<false>& b, f32x16 c) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.v, b.v, c, 0, 0, 0, a.e, 0, b.e);
+}
+__device__ __forceinline__ f32x16 mfma_blocks(const Frag<true>& a, const Frag<true>& b, f32x16 c) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v[q], b.v[q], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ i32x8 codes32(const uint8_t* lo, const uint8_t* hi) {
+  return __builtin_shufflevector(*reinterpret_cast<const i32x4*>(lo), *reinterpret_cast<const i32x4*>(hi), 0, 1, 2, 3, 4,
+                                 5, 6, 7);
 }
 
 template <typename C>
@@ -306,108 +318,224 @@ __device__ __forceinline__ f32x4 bias4(const float* b, int n, int N) {
   return v;
 }
 
-// 16-B-per-lane LDS-DMA (lane l lands at lds_byte + 16 l); the wait is the caller's
-__device__ __forceinline__ void glds16(const void* gsrc, unsigned lds_byte) {
-  unsigned keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep)
-               : "v"(gsrc), "s"(lds_byte)
-               : "memory");
+// LDS-DMA of 16 bytes a lane from base + off; lane l lands at lds_byte + 16 l.
+// The wait is the caller's: the compiler does not know of the load.
+__device__ __forceinline__ void glds16(const uint8_t* base, uint32_t off, unsigned lds_byte) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(base), "s"(lds_byte)
+               : "memory", "m0");
 }
 __device__ __forceinline__ unsigned lds_addr(const void* p) {
   return (unsigned)(uintptr_t)((const __attribute__((address_space(3))) char*)p);
 }
+__device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
-// Output tile of WR x WC waves, each MT x NT instruction tiles.  The matrix
+// Output tile of WR x WC waves, each MT x NT instruction tiles of 32 x 32.  The
 // instruction's rows are b's (columns of the output), its columns a's: a lane
-// then holds 4 consecutive outputs of one row.  LDS: two buffers of BM + BN
-// rows of 128 bytes, filled by LDS-DMA one block ahead; 16-byte piece p of row
-// r sits at place p ^ (r & 7), so the 16 rows that a fragment read touches
-// spread over the banks (the DMA writes lanes in order, so the turn is made in
-// the global address).
+// then holds runs of 4 consecutive outputs of one row.
+//
+// LDS holds two blocks of K (BM + BN rows of 128 bytes each), filled by
+// LDS-DMA.  16-byte piece p of row r sits at place p ^ ((r / 2) & 7), so that
+// 16 rows' pieces, which a fragment read takes in one cycle, spread over all
+// 64 banks; the DMA writes lanes in order, so the turn is made in the global
+// address.
+//
+// A block is used in two halves of 64.  While one half's instructions run, the
+// next half's fragments come from LDS into registers; between the halves all
+// waves have taken what they need of this buffer and the next one has landed,
+// so one barrier a block both frees this buffer, for the block after the next,
+// and opens the other.  A block's DMA thus has one block's time to arrive.
 template <int WR, int WC, int MT, int NT, typename C>
 __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
   using F = Frag<std::is_same<C, float>::value>;
-  constexpr int BM = WR * MT * 16, BN = WC * NT * 16, W = WR * WC, ROWS = BM + BN;
+  constexpr int BM = WR * MT * 32, BN = WC * NT * 32, W = WR * WC, ROWS = BM + BN;
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][ROWS * 128];
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wr = w / WC, wc = w % WC;
-  const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
+  // the 8 XCDs take workgroups in turn: give each a run of tiles, 8 rows of tiles deep, that share operands in its L2
+  const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN, tiles = tm * tn;
+  const int q = tiles / 8, rr = tiles % 8, xcd = blockIdx.x % 8;
+  const int id = (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + blockIdx.x / 8;
+  const int band = id / (8 * tn), deep = min(8, tm - band * 8), in = id - band * 8 * tn;
+  const int m0 = (band * 8 + in % deep) * BM, n0 = in / deep * BN;
   const int64_t kp = fp8_kp(g.K), sp = fp8_sp(g.K);
   const int nb = (int)(kp / 128), per = (nb + g.ksplit - 1) / g.ksplit;
   const int kb0 = blockIdx.z * per, kb1 = min(nb, kb0 + per);
-  constexpr int LOADS = ROWS / 8 / W;  // each fills 8 rows
-  static_assert(ROWS % (8 * W) == 0 && BM % 8 == 0, "whole loads");
-  const uint8_t* src[LOADS];
+  constexpr int LA = BM / 8 / W, LB = BN / 8 / W;  // DMAs of 8 rows a wave
+  static_assert(BM % (8 * W) == 0 && BN % (8 * W) == 0, "whole loads");
+  const uint8_t *ga = g.a + m0 * kp, *gb = g.b + n0 * kp;
+  uint32_t offa[LA], offb[LB];
+  static_assert(W % 2 == 0, "a wave's DMAs all start at rows of one parity of 8");
+  const int lr = lane >> 3, piece = ((lane & 7) ^ ((w & 1) * 4 + (lr >> 1))) * 16;
+  // rows past the end read the last one: their outputs are not stored
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    const int r = (i * W + w) * 8 + (lane >> 3), piece = (lane & 7) ^ (r & 7);
-    // rows past the end read the last one: their outputs are not stored
-    const int64_t row = r < BM ? min(m0 + r, g.M - 1) : min(n0 + r - BM, g.N - 1);
-    src[i] = (r < BM ? g.a : g.b) + row * kp + piece * 16 + (int64_t)kb0 * 128;
-  }
-  auto fill = [&](int buf) {
+  for (int i = 0; i < LA; ++i) offa[i] = (uint32_t)(min((i * W + w) * 8 + lr, g.M - 1 - m0) * kp) + piece;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      glds16(src[i], __builtin_amdgcn_readfirstlane(lds_addr(&lds[buf][(i * W + w) * 1024])));
-      src[i] += 128;
-    }
+  for (int i = 0; i < LB; ++i) offb[i] = (uint32_t)(min((i * W + w) * 8 + lr, g.N - 1 - n0) * kp) + piece;
+  const unsigned base = lds_addr(&lds[0][0]) + w * 1024;
+  auto fill = [&](int buf, int kb) {  // past the last block: that one again, unused
+    const uint8_t *pa = ga + min(kb, kb1 - 1) * 128, *pb = gb + min(kb, kb1 - 1) * 128;
+#pragma unroll
+    for (int i = 0; i < LA; ++i) glds16(pa, offa[i], base + buf * (ROWS * 128) + i * W * 1024);
+#pragma unroll
+    for (int i = 0; i < LB; ++i) glds16(pb, offb[i], base + buf * (ROWS * 128) + BM * 128 + i * W * 1024);
   };
-  const int fr = lane & 15, fg = lane >> 4;
+  const int fr = lane & 31, fh = lane >> 5;
   const uint8_t *psa[MT], *psb[NT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) psa[i] = g.sa + (int64_t)min(m0 + (wr * MT + i) * 16 + fr, g.M - 1) * sp;
+  for (int i = 0; i < MT; ++i) psa[i] = g.sa + (int64_t)min(m0 + (wr * MT + i) * 32 + fr, g.M - 1) * sp;
 #pragma unroll
-  for (int i = 0; i < NT; ++i) psb[i] = g.sb + (int64_t)min(n0 + (wc * NT + i) * 16 + fr, g.N - 1) * sp;
-  uint32_t sa[MT], sb[NT];
-  f32x4 acc[MT][NT];
+  for (int i = 0; i < NT; ++i) psb[i] = g.sb + (int64_t)min(n0 + (wc * NT + i) * 32 + fr, g.N - 1) * sp;
+  uint32_t sa[MT], sb[NT], na[MT], nb4[NT];  // exponent bytes of four blocks at once, and of the next four
+  auto scales = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) na[i] = *reinterpret_cast<const uint32_t*>(psa[i] + (kb & ~3));
+#pragma unroll
+    for (int i = 0; i < NT; ++i) nb4[i] = *reinterpret_cast<const uint32_t*>(psb[i] + (kb & ~3));
+  };
+  // right after wait_all(): the compiler's own wait for these loads falls here, where it costs nothing, and not on the
+  // DMAs that are issued next
+  auto landed = [&]() {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(na[i]));
+#pragma unroll
+    for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(nb4[i]));
+  };
+  auto turn = [&]() {
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sa[i] = na[i];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) sb[i] = nb4[i];
+  };
+  f32x16 acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto frag = [&](int buf, int row, uint32_t byte) {
-    const uint8_t* p = &lds[buf][row * 128];
-    return F(*reinterpret_cast<const i32x4*>(p + ((fg ^ (row & 7)) * 16)),
-             *reinterpret_cast<const i32x4*>(p + (((fg + 4) ^ (row & 7)) * 16)), byte);
-  };
-  if (kb0 < kb1) fill(0);
-  for (int kb = kb0; kb < kb1; ++kb) {
-    const int buf = (kb - kb0) & 1;
-    if (kb == kb0 || (kb & 3) == 0) {
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) sa[i] = *reinterpret_cast<const uint32_t*>(psa[i] + (kb & ~3));
-#pragma unroll
-      for (int i = 0; i < NT; ++i) sb[i] = *reinterpret_cast<const uint32_t*>(psb[i] + (kb & ~3));
-    }
-    // this wave's part of the buffer has arrived; after the barrier everybody's has, and nobody reads the other one
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (kb + 1 < kb1) fill(buf ^ 1);
-    const int sh = (kb & 3) * 8;
-    F fb[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) fb[j] = frag(buf, BM + (wc * NT + j) * 16 + fr, sb[j] >> sh & 0xffu);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const F fa = frag(buf, (wr * MT + i) * 16 + fr, sa[i] >> sh & 0xffu);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = mfma_blocks(fb[j], fa, acc[i][j]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int m = m0 + (wr * MT + i) * 16 + fr;
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  i32x8 fa[2][MT], fb[2][NT];  // of the two halves
+  const uint8_t* fbase = &lds[0][(wr * MT * 32 + fr) * 128];
+  const uint8_t* gbase = &lds[0][(BM + wc * NT * 32 + fr) * 128];
+  auto read = [&](int buf, int h) {
+    const int p0 = ((h * 4 + fh) ^ (fr >> 1 & 7)) * 16, p1 = ((h * 4 + fh + 2) ^ (fr >> 1 & 7)) * 16;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      const int n = n0 + (wc * NT + j) * 16 + fg * 4;
-      if (m >= g.M || n >= g.N) continue;
-      if (g.ksplit > 1) {
-        store4(g.slab + ((int64_t)blockIdx.z * g.M + m) * g.N + n, g.N - n, acc[i][j]);
-      } else {
-        store4((C*)g.c + (int64_t)m * g.N + n, g.N - n, acc[i][j] + bias4(g.bias, n, g.N));
+      const uint8_t* p = gbase + buf * (ROWS * 128) + j * 32 * 128;
+      fb[h][j] = codes32(p + p0, p + p1);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const uint8_t* p = fbase + buf * (ROWS * 128) + i * 32 * 128;
+      fa[h][i] = codes32(p + p0, p + p1);
+    }
+  };
+  auto have = [&](int h) {  // the compiler's wait for this half's reads falls here
+#pragma unroll
+    for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(fb[h][j]));
+#pragma unroll
+    for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(fa[h][i]));
+  };
+  auto multiply = [&](int h, int kb) {
+    const int sh = (kb & 3) * 8;
+    F b[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) b[j] = F(fb[h][j], sb[j] >> sh & 0xffu);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const F a(fa[h][i], sa[i] >> sh & 0xffu);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = mfma_blocks(b[j], a, acc[i][j]);
+    }
+  };
+  scales(kb0);
+  fill(0, kb0);
+  fill(1, kb0 + 1);
+  wait_all();
+  landed();
+  turn();
+  block_barrier();
+  read(0, 0);
+  // The inner loop is one basic block: with a branch in it the compiler gathers both halves' instructions behind the
+  // barrier.  The exponent bytes come once in four blocks: a row's are far from the next row's, so each load touches 32
+  // lines, and a load a block took as long as the codes' DMA.
+  for (int kb = kb0; kb < kb1;) {
+    const int end = min((kb & ~3) + 4, kb1);
+    scales(min(end, kb1 - 1));
+    for (; kb < end; ++kb) {
+      const int buf = (kb - kb0) & 1;
+      have(0);
+      read(buf, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(0, kb);
+      __builtin_amdgcn_sched_barrier(0);
+      wait_all();
+      landed();
+      have(1);
+      block_barrier();
+      fill(buf, kb + 2);
+      read(buf ^ 1, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(1, kb);
+    }
+    turn();
+  }
+  wait_all();  // no DMA may outlive its use of LDS
+  block_barrier();
+  // A wave turns its tile through its own part of LDS, so that rows leave in whole lines: 16-byte piece p of row r at
+  // place p ^ r (as far as there are pieces), which spreads both ways over the banks.
+  auto leave = [&](auto out, bool bias) {
+    typedef decltype(out) O;
+    typedef O vec __attribute__((ext_vector_type(16 / sizeof(O)), aligned(sizeof(O))));
+    typedef O vec4 __attribute__((ext_vector_type(4)));
+    constexpr int PER = 16 / sizeof(O), PIECES = NT * 32 / PER, PART = 2 * ROWS * 128 / W;
+    constexpr int STEP = PART / (PIECES * 16) / 32 < MT ? PART / (PIECES * 16) / 32 : MT;  // instruction tiles at a time
+    static_assert(STEP >= 1 && MT % STEP == 0 && 64 % PIECES == 0, "whole passes");
+    uint8_t* mine = &lds[0][0] + w * PART;
+    O* c = g.ksplit > 1 ? (O*)(g.slab + (int64_t)blockIdx.z * g.M * g.N) : (O*)g.c;
+    const int nw = n0 + wc * NT * 32;
+#pragma unroll
+    for (int i0 = 0; i0 < MT; i0 += STEP) {
+#pragma unroll
+      for (int i = 0; i < STEP; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = i * 32 + fr, col = j * 32 + r * 8 + fh * 4;
+            f32x4 v{acc[i0 + i][j][4 * r], acc[i0 + i][j][4 * r + 1], acc[i0 + i][j][4 * r + 2], acc[i0 + i][j][4 * r + 3]};
+            if (bias) v += bias4(g.bias, nw + col, g.N);
+            vec4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = (O)v[e];
+            *reinterpret_cast<vec4*>(mine + row * PIECES * 16 + ((col / PER) ^ (row & (PIECES - 1))) * 16 +
+                                     col % PER * sizeof(O)) = x;
+          }
+      const int mw = m0 + (wr * MT + i0) * 32;
+#pragma unroll 4
+      for (int q = 0; q < STEP * 32 * PIECES / 64; ++q) {
+        const int row = q * (64 / PIECES) + lane / PIECES, piece = lane % PIECES, m = mw + row, n = nw + piece * PER;
+        const vec x = *reinterpret_cast<const vec*>(mine + row * PIECES * 16 + (piece ^ (row & (PIECES - 1))) * 16);
+        if (m >= g.M || n >= g.N) continue;
+        O* p = c + (int64_t)m * g.N + n;
+        if (n + PER <= g.N) {
+          *reinterpret_cast<vec*>(p) = x;
+        } else {
+#pragma unroll
+          for (int e = 0; e < PER; ++e)
+            if (n + e < g.N) p[e] = x[e];
+        }
       }
     }
-  }
+  };
+  if (g.ksplit > 1) leave(float(0), false);
+  else leave(C(0), g.bias != nullptr);
 }
 
 // c = sum of the slices in order (+ bias)
@@ -455,9 +583,7 @@ __global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
     acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   using F = Frag<std::is_same<C, float>::value>;
-  auto load = [](const uint8_t* p, uint32_t byte) {
-    return F(*reinterpret_cast<const i32x4*>(p), *reinterpret_cast<const i32x4*>(p + 16), byte);
-  };
+  auto load = [](const uint8_t* p, uint32_t byte) { return F(codes32(p, p + 16), byte); };
   for (int kb = w; kb < nb; kb += 8) {
     const F fb = load(pb + (int64_t)kb * 128, psb[kb]);
 #pragma unroll
@@ -484,8 +610,12 @@ void gemm(const Fp8GemmArgs& g, hipStream_t s) {
     else hipLaunchKernelGGL((k_fp8_skinny<4, C>), grid, dim3(512), 0, s, g);
     return;
   }
-  const dim3 grid((g.N + 127) / 128, (g.M + 127) / 128, g.ksplit);
-  hipLaunchKernelGGL((k_fp8_gemm<2, 2, 4, 4, C>), grid, dim3(256), 0, s, g);
+  auto tiles = [&](int bm, int bn) { return dim3((unsigned)((int64_t)((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn)), 1, g.ksplit); };
+  if ((int64_t)g.M * g.N >= (int64_t)256 * 256 * 192) {
+    hipLaunchKernelGGL((k_fp8_gemm<2, 2, 4, 4, C>), tiles(256, 256), dim3(256), 0, s, g);
+  } else {
+    hipLaunchKernelGGL((k_fp8_gemm<2, 2, 2, 2, C>), tiles(128, 128), dim3(256), 0, s, g);
+  }
   if (g.ksplit > 1) {
     const int64_t n = ((int64_t)g.N + 3) / 4 * g.M;
     hipLaunchKernelGGL(k_fp8_join<C>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, g);
