@@ -329,7 +329,17 @@ __device__ __forceinline__ void glds16(const uint8_t* base, uint32_t off, unsign
 __device__ __forceinline__ unsigned lds_addr(const void* p) {
   return (unsigned)(uintptr_t)((const __attribute__((address_space(3))) char*)p);
 }
-__device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void glds4(const uint8_t* base, uint32_t off, unsigned lds_byte) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
+               :
+               : "v"(off), "s"(base), "s"(lds_byte)
+               : "memory", "m0");
+}
+// all but the newest N loads and DMAs of this wave are done, and all its LDS reads
+template <int N>
+__device__ __forceinline__ void wait_but() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
 __device__ __forceinline__ void block_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -340,22 +350,21 @@ __device__ __forceinline__ void block_barrier() {
 // instruction's rows are b's (columns of the output), its columns a's: a lane
 // then holds runs of 4 consecutive outputs of one row.
 //
-// LDS holds two blocks of K (BM + BN rows of 128 bytes each), filled by
-// LDS-DMA.  16-byte piece p of row r sits at place p ^ ((r / 2) & 7), so that
-// 16 rows' pieces, which a fragment read takes in one cycle, spread over all
-// 64 banks; the DMA writes lanes in order, so the turn is made in the global
-// address.
-//
-// A block is used in two halves of 64.  While one half's instructions run, the
-// next half's fragments come from LDS into registers; between the halves all
-// waves have taken what they need of this buffer and the next one has landed,
-// so one barrier a block both frees this buffer, for the block after the next,
-// and opens the other.  A block's DMA thus has one block's time to arrive.
+// K goes by in steps of 64.  LDS is a ring of four steps (BM + BN rows of 64
+// bytes each), filled by LDS-DMA.  While a step's instructions run, the next
+// step's fragments come from LDS into registers; when all waves have them, one
+// barrier a step frees their place for the step after the next three, so a
+// DMA has three steps' time to arrive.  16-byte piece p of row r sits at place
+// p ^ ((r / 4) & 3): the 16 rows that a fragment read takes in one cycle then
+// spread over all 64 banks; the DMA writes lanes in order, so the turn is made
+// in the global address.  The exponent bytes come by DMA too, the dwords of
+// four blocks at once and four blocks ahead.
 template <int WR, int WC, int MT, int NT, typename C>
 __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
   using F = Frag<std::is_same<C, float>::value>;
-  constexpr int BM = WR * MT * 32, BN = WC * NT * 32, W = WR * WC, ROWS = BM + BN;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][ROWS * 128];
+  constexpr int BM = WR * MT * 32, BN = WC * NT * 32, W = WR * WC, ROWS = BM + BN, STEP = ROWS * 64;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * STEP];
+  __shared__ uint32_t words[2][ROWS];
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wr = w / WC, wc = w % WC;
   // the 8 XCDs take workgroups in turn: give each a run of tiles, 8 rows of tiles deep, that share operands in its L2
@@ -365,53 +374,46 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
   const int band = id / (8 * tn), deep = min(8, tm - band * 8), in = id - band * 8 * tn;
   const int m0 = (band * 8 + in % deep) * BM, n0 = in / deep * BN;
   const int64_t kp = fp8_kp(g.K), sp = fp8_sp(g.K);
-  const int nb = (int)(kp / 128), per = (nb + g.ksplit - 1) / g.ksplit;
-  const int kb0 = blockIdx.z * per, kb1 = min(nb, kb0 + per);
-  constexpr int LA = BM / 8 / W, LB = BN / 8 / W;  // DMAs of 8 rows a wave
-  static_assert(BM % (8 * W) == 0 && BN % (8 * W) == 0, "whole loads");
+  const int nb = (int)(kp / 128), per = fp8_slice(nb, g.ksplit);
+  const int kb0 = blockIdx.z * per, kb1 = min(nb, kb0 + per);  // kb0 is a multiple of 4; no slice is empty
+  constexpr int LA = BM / 16 / W, LB = BN / 16 / W;            // DMAs of 16 rows a wave and step
+  static_assert(BM % (16 * W) == 0 && BN % (16 * W) == 0, "whole loads");
+  constexpr int LS = ROWS / 64 / W;  // DMAs of 64 dwords a wave and four blocks
+  static_assert(BM == BN && W % 2 == 0 && ROWS % (64 * W) == 0, "a wave's dwords are all of one operand");
   const uint8_t *ga = g.a + m0 * kp, *gb = g.b + n0 * kp;
-  uint32_t offa[LA], offb[LB];
-  static_assert(W % 2 == 0, "a wave's DMAs all start at rows of one parity of 8");
-  const int lr = lane >> 3, piece = ((lane & 7) ^ ((w & 1) * 4 + (lr >> 1))) * 16;
+  uint32_t offa[LA], offb[LB], offs[LS];
+  const int lr = lane >> 2, piece = ((lane & 3) ^ (lane >> 4)) * 16;
   // rows past the end read the last one: their outputs are not stored
 #pragma unroll
-  for (int i = 0; i < LA; ++i) offa[i] = (uint32_t)(min((i * W + w) * 8 + lr, g.M - 1 - m0) * kp) + piece;
+  for (int i = 0; i < LA; ++i) offa[i] = (uint32_t)(min((i * W + w) * 16 + lr, g.M - 1 - m0) * kp) + piece;
 #pragma unroll
-  for (int i = 0; i < LB; ++i) offb[i] = (uint32_t)(min((i * W + w) * 8 + lr, g.N - 1 - n0) * kp) + piece;
-  const unsigned base = lds_addr(&lds[0][0]) + w * 1024;
-  auto fill = [&](int buf, int kb) {  // past the last block: that one again, unused
-    const uint8_t *pa = ga + min(kb, kb1 - 1) * 128, *pb = gb + min(kb, kb1 - 1) * 128;
+  for (int i = 0; i < LB; ++i) offb[i] = (uint32_t)(min((i * W + w) * 16 + lr, g.N - 1 - n0) * kp) + piece;
+  const bool of_b = w >= W / 2;
+  const uint8_t* gs = of_b ? g.sb + n0 * sp : g.sa + m0 * sp;
 #pragma unroll
-    for (int i = 0; i < LA; ++i) glds16(pa, offa[i], base + buf * (ROWS * 128) + i * W * 1024);
+  for (int i = 0; i < LS; ++i)
+    offs[i] = (uint32_t)(min((w % (W / 2) * LS + i) * 64 + lane, (of_b ? g.N - n0 : g.M - m0) - 1) * sp);
+  const unsigned base = lds_addr(lds) + w * 1024, base_s = lds_addr(words) + w * LS * 256;
+  auto fill_part = [&](int slot, int step, int i) {  // DMA i of a step's; past the last step: that one again, unused
+    const int at = min(step, 2 * kb1 - 1) * 64;
+    if (i < LA) glds16(ga + at, offa[i], base + slot * STEP + i * W * 1024);
+    else glds16(gb + at, offb[i - LA], base + slot * STEP + BM * 64 + (i - LA) * W * 1024);
+  };
+  auto fill = [&](int slot, int step) {
 #pragma unroll
-    for (int i = 0; i < LB; ++i) glds16(pb, offb[i], base + buf * (ROWS * 128) + BM * 128 + i * W * 1024);
+    for (int i = 0; i < LA + LB; ++i) fill_part(slot, step, i);
+  };
+  auto fill_words = [&](int kb) {  // of the four blocks that kb begins
+#pragma unroll
+    for (int i = 0; i < LS; ++i) glds4(gs + min(kb, kb1 - 1) / 4 * 4, offs[i], base_s + (kb >> 2 & 1) * (ROWS * 4) + i * 256);
   };
   const int fr = lane & 31, fh = lane >> 5;
-  const uint8_t *psa[MT], *psb[NT];
+  uint32_t sa[MT], sb[NT];
+  auto read_words = [&](int kb) {
 #pragma unroll
-  for (int i = 0; i < MT; ++i) psa[i] = g.sa + (int64_t)min(m0 + (wr * MT + i) * 32 + fr, g.M - 1) * sp;
+    for (int i = 0; i < MT; ++i) sa[i] = words[kb >> 2 & 1][(wr * MT + i) * 32 + fr];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) psb[i] = g.sb + (int64_t)min(n0 + (wc * NT + i) * 32 + fr, g.N - 1) * sp;
-  uint32_t sa[MT], sb[NT], na[MT], nb4[NT];  // exponent bytes of four blocks at once, and of the next four
-  auto scales = [&](int kb) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) na[i] = *reinterpret_cast<const uint32_t*>(psa[i] + (kb & ~3));
-#pragma unroll
-    for (int i = 0; i < NT; ++i) nb4[i] = *reinterpret_cast<const uint32_t*>(psb[i] + (kb & ~3));
-  };
-  // right after wait_all(): the compiler's own wait for these loads falls here, where it costs nothing, and not on the
-  // DMAs that are issued next
-  auto landed = [&]() {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(na[i]));
-#pragma unroll
-    for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(nb4[i]));
-  };
-  auto turn = [&]() {
-#pragma unroll
-    for (int i = 0; i < MT; ++i) sa[i] = na[i];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) sb[i] = nb4[i];
+    for (int j = 0; j < NT; ++j) sb[j] = words[kb >> 2 & 1][BM + (wc * NT + j) * 32 + fr];
   };
   f32x16 acc[MT][NT];
 #pragma unroll
@@ -420,30 +422,31 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  i32x8 fa[2][MT], fb[2][NT];  // of the two halves
-  const uint8_t* fbase = &lds[0][(wr * MT * 32 + fr) * 128];
-  const uint8_t* gbase = &lds[0][(BM + wc * NT * 32 + fr) * 128];
-  auto read = [&](int buf, int h) {
-    const int p0 = ((h * 4 + fh) ^ (fr >> 1 & 7)) * 16, p1 = ((h * 4 + fh + 2) ^ (fr >> 1 & 7)) * 16;
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const uint8_t* p = gbase + buf * (ROWS * 128) + j * 32 * 128;
-      fb[h][j] = codes32(p + p0, p + p1);
-    }
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const uint8_t* p = fbase + buf * (ROWS * 128) + i * 32 * 128;
-      fa[h][i] = codes32(p + p0, p + p1);
-    }
+  i32x8 fa[2][MT], fb[2][NT];  // of this step and the next
+  const int p0 = ((fh * 2) ^ (fr >> 2 & 3)) * 16, p1 = ((fh * 2 + 1) ^ (fr >> 2 & 3)) * 16;
+  const uint8_t *fbase = lds + (wr * MT * 32 + fr) * 64, *gbase = lds + (BM + wc * NT * 32 + fr) * 64;
+  auto read_a = [&](int slot, int h, int i) {
+    const uint8_t* p = fbase + slot * STEP + i * 32 * 64;
+    fa[h][i] = codes32(p + p0, p + p1);
   };
-  auto have = [&](int h) {  // the compiler's wait for this half's reads falls here
+  auto read_b = [&](int slot, int h, int j) {
+    const uint8_t* p = gbase + slot * STEP + j * 32 * 64;
+    fb[h][j] = codes32(p + p0, p + p1);
+  };
+  auto have = [&](int h) {  // the compiler's wait for these fragments falls here
 #pragma unroll
     for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(fb[h][j]));
 #pragma unroll
     for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(fa[h][i]));
   };
-  auto multiply = [&](int h, int kb) {
-    const int sh = (kb & 3) * 8;
+  constexpr int LOADS = LA + LB, GAPS = MT > 1 ? MT - 1 : 1;
+  // step `step` from fragments h, its place in the ring `slot`; the next one's reads and a DMA go between the rows of
+  // instructions, none behind the last row, where the reads would be waited for
+  auto run = [&](int step, int slot, int next, int h) {
+    const int sh = (step >> 1 & 3) * 8;
+    wait_but<2 * LOADS>();  // the next step has landed
+    have(h);
+    block_barrier();
     F b[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) b[j] = F(fb[h][j], sb[j] >> sh & 0xffu);
@@ -452,41 +455,39 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
       const F a(fa[h][i], sa[i] >> sh & 0xffu);
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = mfma_blocks(b[j], a, acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i >= GAPS) continue;
+#pragma unroll
+      for (int l = i * NT / GAPS; l < (i + 1) * NT / GAPS; ++l) read_b(next, h ^ 1, l);
+#pragma unroll
+      for (int l = i * MT / GAPS; l < (i + 1) * MT / GAPS; ++l) read_a(next, h ^ 1, l);
+#pragma unroll
+      for (int l = i * LOADS / GAPS; l < (i + 1) * LOADS / GAPS; ++l) fill_part(slot, step + 4, l);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  scales(kb0);
-  fill(0, kb0);
-  fill(1, kb0 + 1);
-  wait_all();
-  landed();
-  turn();
+  fill_words(kb0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) fill(i, 2 * kb0 + i);
+  wait_but<3 * LOADS>();
   block_barrier();
-  read(0, 0);
-  // The inner loop is one basic block: with a branch in it the compiler gathers both halves' instructions behind the
-  // barrier.  The exponent bytes come once in four blocks: a row's are far from the next row's, so each load touches 32
-  // lines, and a load a block took as long as the codes' DMA.
+  read_words(kb0);
+#pragma unroll
+  for (int j = 0; j < NT; ++j) read_b(0, 0, j);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) read_a(0, 0, i);
+  // the inner loop is one basic block: the compiler moves matrix instructions over a barrier to where a branch ends
   for (int kb = kb0; kb < kb1;) {
-    const int end = min((kb & ~3) + 4, kb1);
-    scales(min(end, kb1 - 1));
+    const int end = min(kb + 4, kb1);
+    fill_words(kb + 4);
     for (; kb < end; ++kb) {
-      const int buf = (kb - kb0) & 1;
-      have(0);
-      read(buf, 1);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(0, kb);
-      __builtin_amdgcn_sched_barrier(0);
-      wait_all();
-      landed();
-      have(1);
-      block_barrier();
-      fill(buf, kb + 2);
-      read(buf ^ 1, 0);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(1, kb);
+      const int slot = (kb - kb0 & 1) * 2;
+      run(2 * kb, slot, slot + 1, 0);
+      run(2 * kb + 1, slot + 1, slot ^ 2, 1);
     }
-    turn();
+    read_words(kb);
   }
-  wait_all();  // no DMA may outlive its use of LDS
+  wait_but<0>();  // no DMA may outlive its use of LDS
   block_barrier();
   // A wave turns its tile through its own part of LDS, so that rows leave in whole lines: 16-byte piece p of row r at
   // place p ^ r (as far as there are pieces), which spreads both ways over the banks.
@@ -494,16 +495,16 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
     typedef decltype(out) O;
     typedef O vec __attribute__((ext_vector_type(16 / sizeof(O)), aligned(sizeof(O))));
     typedef O vec4 __attribute__((ext_vector_type(4)));
-    constexpr int PER = 16 / sizeof(O), PIECES = NT * 32 / PER, PART = 2 * ROWS * 128 / W;
-    constexpr int STEP = PART / (PIECES * 16) / 32 < MT ? PART / (PIECES * 16) / 32 : MT;  // instruction tiles at a time
-    static_assert(STEP >= 1 && MT % STEP == 0 && 64 % PIECES == 0, "whole passes");
-    uint8_t* mine = &lds[0][0] + w * PART;
+    constexpr int PER = 16 / sizeof(O), PIECES = NT * 32 / PER, PART = 4 * STEP / W;
+    constexpr int TILES = PART / (PIECES * 16) / 32 < MT ? PART / (PIECES * 16) / 32 : MT;  // instruction tiles at a time
+    static_assert(TILES >= 1 && MT % TILES == 0 && 64 % PIECES == 0, "whole passes");
+    uint8_t* mine = lds + w * PART;
     O* c = g.ksplit > 1 ? (O*)(g.slab + (int64_t)blockIdx.z * g.M * g.N) : (O*)g.c;
     const int nw = n0 + wc * NT * 32;
 #pragma unroll
-    for (int i0 = 0; i0 < MT; i0 += STEP) {
+    for (int i0 = 0; i0 < MT; i0 += TILES) {
 #pragma unroll
-      for (int i = 0; i < STEP; ++i)
+      for (int i = 0; i < TILES; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -519,7 +520,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
           }
       const int mw = m0 + (wr * MT + i0) * 32;
 #pragma unroll 4
-      for (int q = 0; q < STEP * 32 * PIECES / 64; ++q) {
+      for (int q = 0; q < TILES * 32 * PIECES / 64; ++q) {
         const int row = q * (64 / PIECES) + lane / PIECES, piece = lane % PIECES, m = mw + row, n = nw + piece * PER;
         const vec x = *reinterpret_cast<const vec*>(mine + row * PIECES * 16 + (piece ^ (row & (PIECES - 1))) * 16);
         if (m >= g.M || n >= g.N) continue;
@@ -631,7 +632,7 @@ int fp8_gemm_ksplit(int M, int N, int64_t K) {
   int64_t split = 256 / tiles;
   if (split > nb / 4) split = nb / 4;
   if (split < 1) split = 1;
-  const int64_t per = (nb + split - 1) / split;
+  const int per = fp8_slice((int)nb, (int)split);
   return (int)((nb + per - 1) / per);  // no empty slice
 }
 

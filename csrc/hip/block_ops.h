@@ -102,6 +102,8 @@ struct Fp8GemmArgs {  // c [M, N] = a [M, K] b [N, K]^T (+ bias [N])
   int ksplit = 1;         // slices of K; more than one goes through the slab
   float* slab = nullptr;  // [ksplit][M][N]
 };
+// blocks of a slice: a multiple of 4, as the exponent bytes' dwords are
+PBX_FP8_HD int fp8_slice(int blocks, int ksplit) { return ((blocks + ksplit - 1) / ksplit + 3) / 4 * 4; }
 int fp8_gemm_ksplit(int M, int N, int64_t K);
 void launch_fp8_gemm(const Fp8GemmArgs& a, hipStream_t s);
 
