@@ -335,11 +335,8 @@ __device__ __forceinline__ void glds4(const uint8_t* base, uint32_t off, unsigne
                : "v"(off), "s"(base), "s"(lds_byte)
                : "memory", "m0");
 }
-// all but the newest N loads and DMAs of this wave are done, and all its LDS reads
-template <int N>
-__device__ __forceinline__ void wait_but() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
-}
+// all loads, DMAs and LDS reads of this wave are done
+__device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void block_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -350,20 +347,25 @@ __device__ __forceinline__ void block_barrier() {
 // instruction's rows are b's (columns of the output), its columns a's: a lane
 // then holds runs of 4 consecutive outputs of one row.
 //
-// K goes by in steps of 64.  LDS is a ring of four steps (BM + BN rows of 64
-// bytes each), filled by LDS-DMA.  While a step's instructions run, the next
-// step's fragments come from LDS into registers; when all waves have them, one
-// barrier a step frees their place for the step after the next three, so a
-// DMA has three steps' time to arrive.  16-byte piece p of row r sits at place
-// p ^ ((r / 4) & 3): the 16 rows that a fragment read takes in one cycle then
-// spread over all 64 banks; the DMA writes lanes in order, so the turn is made
-// in the global address.  The exponent bytes come by DMA too, the dwords of
-// four blocks at once and four blocks ahead.
+// LDS holds two blocks of K (BM + BN rows of 128 bytes each), filled by
+// LDS-DMA in whole lines (rows of 64 bytes at a time took twice the requests
+// of the L2 and bounded the kernel).  A block is used in two halves of 64:
+// while one half's instructions run, the next one's fragments come from LDS
+// into registers.  Before the last row of the first half's instructions all
+// waves have the second half's fragments and the next block has landed: one
+// barrier a block, there, frees this block's place for the block after the
+// next, whose DMA then has nearly a block's time to arrive.
+//
+// 16-byte piece p of row r sits at place p ^ ((r / 2) & 7): the 16 rows that a
+// fragment read takes in one cycle then spread over all 64 banks; the DMA
+// writes lanes in order, so the turn is made in the global address.  The
+// exponent bytes come by DMA too, the dwords of four blocks at once and four
+// blocks ahead.
 template <int WR, int WC, int MT, int NT, typename C>
 __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
   using F = Frag<std::is_same<C, float>::value>;
-  constexpr int BM = WR * MT * 32, BN = WC * NT * 32, W = WR * WC, ROWS = BM + BN, STEP = ROWS * 64;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * STEP];
+  constexpr int BM = WR * MT * 32, BN = WC * NT * 32, W = WR * WC, ROWS = BM + BN, BLOCK = ROWS * 128;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BLOCK];
   __shared__ uint32_t words[2][ROWS];
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wr = w / WC, wc = w % WC;
@@ -376,32 +378,32 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
   const int64_t kp = fp8_kp(g.K), sp = fp8_sp(g.K);
   const int nb = (int)(kp / 128), per = fp8_slice(nb, g.ksplit);
   const int kb0 = blockIdx.z * per, kb1 = min(nb, kb0 + per);  // kb0 is a multiple of 4; no slice is empty
-  constexpr int LA = BM / 16 / W, LB = BN / 16 / W;            // DMAs of 16 rows a wave and step
-  static_assert(BM % (16 * W) == 0 && BN % (16 * W) == 0, "whole loads");
+  constexpr int LA = BM / 8 / W, LB = BN / 8 / W;              // DMAs of 8 rows a wave and block
+  static_assert(BM % (8 * W) == 0 && BN % (8 * W) == 0, "whole loads");
   constexpr int LS = ROWS / 64 / W;  // DMAs of 64 dwords a wave and four blocks
   static_assert(BM == BN && W % 2 == 0 && ROWS % (64 * W) == 0, "a wave's dwords are all of one operand");
   const uint8_t *ga = g.a + m0 * kp, *gb = g.b + n0 * kp;
   uint32_t offa[LA], offb[LB], offs[LS];
-  const int lr = lane >> 2, piece = ((lane & 3) ^ (lane >> 4)) * 16;
+  const int lr = lane >> 3, piece = ((lane & 7) ^ ((w & 1) * 4 + (lr >> 1))) * 16;  // a wave's rows begin at 8 w, mod 16
   // rows past the end read the last one: their outputs are not stored
 #pragma unroll
-  for (int i = 0; i < LA; ++i) offa[i] = (uint32_t)(min((i * W + w) * 16 + lr, g.M - 1 - m0) * kp) + piece;
+  for (int i = 0; i < LA; ++i) offa[i] = (uint32_t)(min((i * W + w) * 8 + lr, g.M - 1 - m0) * kp) + piece;
 #pragma unroll
-  for (int i = 0; i < LB; ++i) offb[i] = (uint32_t)(min((i * W + w) * 16 + lr, g.N - 1 - n0) * kp) + piece;
+  for (int i = 0; i < LB; ++i) offb[i] = (uint32_t)(min((i * W + w) * 8 + lr, g.N - 1 - n0) * kp) + piece;
   const bool of_b = w >= W / 2;
   const uint8_t* gs = of_b ? g.sb + n0 * sp : g.sa + m0 * sp;
 #pragma unroll
   for (int i = 0; i < LS; ++i)
     offs[i] = (uint32_t)(min((w % (W / 2) * LS + i) * 64 + lane, (of_b ? g.N - n0 : g.M - m0) - 1) * sp);
   const unsigned base = lds_addr(lds) + w * 1024, base_s = lds_addr(words) + w * LS * 256;
-  auto fill_part = [&](int slot, int step, int i) {  // DMA i of a step's; past the last step: that one again, unused
-    const int at = min(step, 2 * kb1 - 1) * 64;
-    if (i < LA) glds16(ga + at, offa[i], base + slot * STEP + i * W * 1024);
-    else glds16(gb + at, offb[i - LA], base + slot * STEP + BM * 64 + (i - LA) * W * 1024);
+  auto fill_part = [&](int buf, int kb, int i) {  // DMA i of a block's; past the last block: that one again, unused
+    const int at = min(kb, kb1 - 1) * 128;
+    if (i < LA) glds16(ga + at, offa[i], base + buf * BLOCK + i * W * 1024);
+    else glds16(gb + at, offb[i - LA], base + buf * BLOCK + BM * 128 + (i - LA) * W * 1024);
   };
-  auto fill = [&](int slot, int step) {
+  auto fill = [&](int buf, int kb) {
 #pragma unroll
-    for (int i = 0; i < LA + LB; ++i) fill_part(slot, step, i);
+    for (int i = 0; i < LA + LB; ++i) fill_part(buf, kb, i);
   };
   auto fill_words = [&](int kb) {  // of the four blocks that kb begins
 #pragma unroll
@@ -422,16 +424,17 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  i32x8 fa[2][MT], fb[2][NT];  // of this step and the next
-  const int p0 = ((fh * 2) ^ (fr >> 2 & 3)) * 16, p1 = ((fh * 2 + 1) ^ (fr >> 2 & 3)) * 16;
-  const uint8_t *fbase = lds + (wr * MT * 32 + fr) * 64, *gbase = lds + (BM + wc * NT * 32 + fr) * 64;
-  auto read_a = [&](int slot, int h, int i) {
-    const uint8_t* p = fbase + slot * STEP + i * 32 * 64;
-    fa[h][i] = codes32(p + p0, p + p1);
-  };
-  auto read_b = [&](int slot, int h, int j) {
-    const uint8_t* p = gbase + slot * STEP + j * 32 * 64;
-    fb[h][j] = codes32(p + p0, p + p1);
+  i32x8 fa[2][MT], fb[2][NT];  // of the two halves
+  const uint8_t *fbase = lds + (wr * MT * 32 + fr) * 128, *gbase = lds + (BM + wc * NT * 32 + fr) * 128;
+  int pos[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) pos[h][e] = ((h * 4 + fh * 2 + e) ^ (fr >> 1 & 7)) * 16;
+  auto read_part = [&](int buf, int h, int l) {  // fragment l of a half's: b's first, all of them are needed at once
+    const uint8_t* p = l < NT ? gbase + l * 32 * 128 : fbase + (l - NT) * 32 * 128;
+    (l < NT ? fb[h][l < NT ? l : 0] : fa[h][l < NT ? 0 : l - NT]) =
+        codes32(p + buf * BLOCK + pos[h][0], p + buf * BLOCK + pos[h][1]);
   };
   auto have = [&](int h) {  // the compiler's wait for these fragments falls here
 #pragma unroll
@@ -439,55 +442,61 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(fa[h][i]));
   };
-  constexpr int LOADS = LA + LB, GAPS = MT > 1 ? MT - 1 : 1;
-  // step `step` from fragments h, its place in the ring `slot`; the next one's reads and a DMA go between the rows of
-  // instructions, none behind the last row, where the reads would be waited for
-  auto run = [&](int step, int slot, int next, int h) {
-    const int sh = (step >> 1 & 3) * 8;
-    wait_but<2 * LOADS>();  // the next step has landed
-    have(h);
-    block_barrier();
-    F b[NT];
+  constexpr int LOADS = LA + LB, FRAGS = MT + NT;
+  // rows [from, to) of half h's instructions; after row i reads share(i) of the fragments of (buf, half) and starts
+  // share(i) of the DMAs, both counted in `gaps` equal shares from row `from`
+  auto rows = [&](const F(&b)[NT], int h, int sh, int from, int to, auto between) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) b[j] = F(fb[h][j], sb[j] >> sh & 0xffu);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int i = from; i < to; ++i) {
       const F a(fa[h][i], sa[i] >> sh & 0xffu);
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = mfma_blocks(b[j], a, acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
-      if (i >= GAPS) continue;
-#pragma unroll
-      for (int l = i * NT / GAPS; l < (i + 1) * NT / GAPS; ++l) read_b(next, h ^ 1, l);
-#pragma unroll
-      for (int l = i * MT / GAPS; l < (i + 1) * MT / GAPS; ++l) read_a(next, h ^ 1, l);
-#pragma unroll
-      for (int l = i * LOADS / GAPS; l < (i + 1) * LOADS / GAPS; ++l) fill_part(slot, step + 4, l);
+      between(i);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  fill_words(kb0);
+  auto spread = [&](int i, int gaps, int n, auto f) {  // share i of n things in `gaps` equal shares
+    if (i < gaps) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) fill(i, 2 * kb0 + i);
-  wait_but<3 * LOADS>();
+      for (int l = i * n / gaps; l < (i + 1) * n / gaps; ++l) f(l);
+    }
+  };
+  constexpr int GAPS = MT > 1 ? MT - 1 : 1, D0 = LOADS / MT;  // DMAs behind the barrier's row
+  auto block = [&](int kb, int buf) {
+    const int sh = (kb & 3) * 8;
+    F b[NT];
+    have(0);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) b[j] = F(fb[0][j], sb[j] >> sh & 0xffu);
+    rows(b, 0, sh, 0, MT - 1, [&](int i) { spread(i, MT > 2 ? MT - 2 : 1, FRAGS, [&](int l) { read_part(buf, 1, l); }); });
+    wait_all();
+    have(1);
+    block_barrier();
+    rows(b, 0, sh, MT - 1, MT, [&](int) { spread(0, 1, D0, [&](int l) { fill_part(buf, kb + 2, l); }); });
+#pragma unroll
+    for (int j = 0; j < NT; ++j) b[j] = F(fb[1][j], sb[j] >> sh & 0xffu);
+    rows(b, 1, sh, 0, MT, [&](int i) {
+      spread(i, GAPS, LOADS - D0, [&](int l) { fill_part(buf, kb + 2, D0 + l); });
+      spread(i, GAPS, FRAGS, [&](int l) { read_part(buf ^ 1, 0, l); });
+    });
+  };
+  fill_words(kb0);
+  fill(0, kb0);
+  fill(1, kb0 + 1);
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
   block_barrier();
   read_words(kb0);
 #pragma unroll
-  for (int j = 0; j < NT; ++j) read_b(0, 0, j);
-#pragma unroll
-  for (int i = 0; i < MT; ++i) read_a(0, 0, i);
+  for (int l = 0; l < FRAGS; ++l) read_part(0, 0, l);
   // the inner loop is one basic block: the compiler moves matrix instructions over a barrier to where a branch ends
   for (int kb = kb0; kb < kb1;) {
     const int end = min(kb + 4, kb1);
     fill_words(kb + 4);
-    for (; kb < end; ++kb) {
-      const int slot = (kb - kb0 & 1) * 2;
-      run(2 * kb, slot, slot + 1, 0);
-      run(2 * kb + 1, slot + 1, slot ^ 2, 1);
-    }
+    for (; kb < end; ++kb) block(kb, kb - kb0 & 1);
     read_words(kb);
   }
-  wait_but<0>();  // no DMA may outlive its use of LDS
+  wait_all();  // no DMA may outlive its use of LDS
   block_barrier();
   // A wave turns its tile through its own part of LDS, so that rows leave in whole lines: 16-byte piece p of row r at
   // place p ^ r (as far as there are pieces), which spreads both ways over the banks.
@@ -495,7 +504,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
     typedef decltype(out) O;
     typedef O vec __attribute__((ext_vector_type(16 / sizeof(O)), aligned(sizeof(O))));
     typedef O vec4 __attribute__((ext_vector_type(4)));
-    constexpr int PER = 16 / sizeof(O), PIECES = NT * 32 / PER, PART = 4 * STEP / W;
+    constexpr int PER = 16 / sizeof(O), PIECES = NT * 32 / PER, PART = 2 * BLOCK / W;
     constexpr int TILES = PART / (PIECES * 16) / 32 < MT ? PART / (PIECES * 16) / 32 : MT;  // instruction tiles at a time
     static_assert(TILES >= 1 && MT % TILES == 0 && 64 % PIECES == 0, "whole passes");
     uint8_t* mine = lds + w * PART;
