@@ -363,7 +363,8 @@ __device__ __forceinline__ void block_barrier() {
 // blocks ahead.
 template <int WR, int WC, int MT, int NT, typename C>
 __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
-  using F = Frag<std::is_same<C, float>::value>;
+  constexpr bool FULL = std::is_same<C, float>::value;
+  using F = Frag<FULL>;
   constexpr int BM = WR * MT * 32, BN = WC * NT * 32, W = WR * WC, ROWS = BM + BN, BLOCK = ROWS * 128;
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BLOCK];
   __shared__ uint32_t words[2][ROWS];
@@ -446,14 +447,24 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
   // rows [from, to) of half h's instructions; after row i reads share(i) of the fragments of (buf, half) and starts
   // share(i) of the DMAs, both counted in `gaps` equal shares from row `from`
   auto rows = [&](const F(&b)[NT], int h, int sh, int from, int to, auto between) {
+    F a(fa[h][from], sa[from] >> sh & 0xffu);
 #pragma unroll
     for (int i = from; i < to; ++i) {
-      const F a(fa[h][i], sa[i] >> sh & 0xffu);
+      F next = a;
+      if (i + 1 < to) next = F(fa[h][i + 1], sa[i + 1] >> sh & 0xffu);
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = mfma_blocks(b[j], a, acc[i][j]);
+      if (FULL && i + 1 < to) {  // the next row's codes become bf16 between this row's instructions
+#pragma unroll
+        for (int k = 0; k < 4 * NT; ++k) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x2, 2, 0);
+        }
+      }
       __builtin_amdgcn_sched_barrier(0);
       between(i);
       __builtin_amdgcn_sched_barrier(0);
+      a = next;
     }
   };
   auto spread = [&](int i, int gaps, int n, auto f) {  // share i of n things in `gaps` equal shares
