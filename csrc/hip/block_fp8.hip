@@ -89,91 +89,193 @@ __global__ __launch_bounds__(256) void k_fp8_quant_rows(Fp8QuantArgs a) {
   }
 }
 
-// One 128 x 128 tile a workgroup, read once: codes in blocks along the rows
-// and, transposed, along the columns, and partial column sums.  Thread t holds
-// columns 4 (t % 32) .. + 3 of rows 16 (t / 32) .. + 15: a row's block is one
-// half-wave, and 16 rows of a column are one 16-byte piece of the transposed
-// codes, put together through LDS so that whole 128-byte lines are written.
+// Eight consecutive values of a row as they lie in memory (16-bit types two to
+// a dword), and what the tile kernel does with them: magnitudes as integers
+// that order like them, and codes straight from the stored type, with the
+// scale in the conversion (v_cvt_scalef32_pk_fp8_*: v / scale, rounded to the
+// nearest, halves to even; what is not finite becomes NaN).
 template <typename E>
-__global__ __launch_bounds__(256) void k_fp8_quant_tile(Fp8QuantArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t cols[128 * 128];
-  __shared__ uint32_t red[8][128];
-  __shared__ uint32_t tile_max[4];
-  const int64_t k0 = (int64_t)blockIdx.x * 128, m0 = (int64_t)blockIdx.y * 128;
-  const int t = threadIdx.x, cq = (t & 31) * 4, rq = t >> 5;
-  const int64_t rows = a.M - m0, width = a.K - k0;
-  const int64_t kp = fp8_kp(a.K), ksp = fp8_sp(a.K), mp = fp8_kp(a.M), msp = fp8_sp(a.M);
-  float v[16][4];
-  const int valid = width - cq >= 4 ? 4 : width - cq > 0 ? (int)(width - cq) : 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = rq * 16 + i;
-    const E* p = (const E*)a.x + (m0 + r) * a.ld + k0 + cq;
-    typedef E vec __attribute__((ext_vector_type(4), aligned(sizeof(E))));
-    if (r < rows && valid == 4) {
-      const vec x = *reinterpret_cast<const vec*>(p);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = (float)x[j];
+struct Eight {
+  typedef E vec8 __attribute__((ext_vector_type(8), aligned(sizeof(E))));
+  typedef E pair __attribute__((ext_vector_type(2)));
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  static constexpr bool WIDE = sizeof(E) == 4;
+  static constexpr int NM = WIDE ? 8 : 4;  // dwords
+  typedef uint32_t dwords __attribute__((ext_vector_type(NM)));
+  dwords d;
+  __device__ __forceinline__ void load(const E* p, int valid) {
+    if (valid >= 8) {
+      d = __builtin_bit_cast(dwords, *reinterpret_cast<const vec8*>(p));
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = r < rows && j < valid ? (float)p[j] : 0.f;
+      for (int k = 0; k < NM; ++k) {
+        if constexpr (WIDE) {
+          d[k] = k < valid ? __builtin_bit_cast(uint32_t, p[k]) : 0u;
+        } else {
+          const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+          const uint32_t lo = 2 * k < valid ? q[2 * k] : 0u, hi = 2 * k + 1 < valid ? q[2 * k + 1] : 0u;
+          d[k] = lo | hi << 16;
+        }
+      }
     }
   }
-  if (a.slab) {
-    float* fr = reinterpret_cast<float*>(red);
+  __device__ __forceinline__ float value(int j) const {
+    if constexpr (WIDE) return __builtin_bit_cast(float, (uint32_t)d[j]);
+    else return (float)__builtin_bit_cast(pair, (uint32_t)d[j / 2])[j & 1];
+  }
+  __device__ __forceinline__ uint32_t mag(int k) const { return d[k] & (WIDE ? 0x7fffffffu : 0x7fff7fffu); }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    if constexpr (WIDE) {
+      return max(a, b);
+    } else {
+      const u16x2 x = __builtin_bit_cast(u16x2, a), y = __builtin_bit_cast(u16x2, b);
+      return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, y));
+    }
+  }
+  // the larger half of a dword of magnitudes, and its bits as fp32
+  static __device__ __forceinline__ uint32_t top(uint32_t m) { return WIDE ? m : max(m & 0xffffu, m >> 16); }
+  static constexpr uint32_t kInf = WIDE ? 0x7f800000u : std::is_same<E, __bf16>::value ? 0x7f80u : 0x7c00u;
+  static __device__ __forceinline__ uint32_t bits(uint32_t m) {
+    if constexpr (WIDE) return m;
+    else if constexpr (std::is_same<E, __bf16>::value) return m << 16;
+    else return __builtin_bit_cast(uint32_t, (float)__builtin_bit_cast(_Float16, (unsigned short)m));
+  }
+  // a dword of magnitudes without those that are not finite
+  static __device__ __forceinline__ uint32_t finite(uint32_t m) {
+    if constexpr (WIDE) return m < kInf ? m : 0u;
+    else return ((m & 0xffffu) < kInf ? m & 0xffffu : 0u) | ((m >> 16) < kInf ? m & 0xffff0000u : 0u);
+  }
+  // codes of two pairs of values, a pair as two dwords of fp32 or the halves of one
+  static __device__ __forceinline__ uint32_t codes(uint32_t a, uint32_t b, uint32_t c, uint32_t e, float scale) {
+    s16x2 r{0, 0};
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, __builtin_bit_cast(float, a), __builtin_bit_cast(float, b), scale, false);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, __builtin_bit_cast(float, c), __builtin_bit_cast(float, e), scale, true);
+    return __builtin_bit_cast(uint32_t, r);
+  }
+  static __device__ __forceinline__ uint32_t codes(uint32_t ab, uint32_t ce, float scale) {
+    s16x2 r{0, 0};
+    if constexpr (std::is_same<E, __bf16>::value) {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(pair, ab), scale, false);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(pair, ce), scale, true);
+    } else {
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(pair, ab), scale, false);
+      r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(pair, ce), scale, true);
+    }
+    return __builtin_bit_cast(uint32_t, r);
+  }
+  __device__ __forceinline__ uint2 row_codes(float scale) const {
+    if constexpr (WIDE) return make_uint2(codes(d[0], d[1], d[2], d[3], scale), codes(d[4], d[5], d[6], d[7], scale));
+    else return make_uint2(codes(d[0], d[1], scale), codes(d[2], d[3], scale));
+  }
+  // of column j of the four rows x[0 .. 3]
+  static __device__ __forceinline__ uint32_t col_codes(const Eight* x, int j, float scale) {
+    if constexpr (WIDE) {
+      return codes(x[0].d[j], x[1].d[j], x[2].d[j], x[3].d[j], scale);
+    } else {
+      const uint32_t sel = j & 1 ? 0x07060302u : 0x05040100u;  // the high or the low halves of two dwords
+      return codes(__builtin_amdgcn_perm(x[1].d[j / 2], x[0].d[j / 2], sel),
+                   __builtin_amdgcn_perm(x[3].d[j / 2], x[2].d[j / 2], sel), scale);
+    }
+  }
+};
+__device__ __forceinline__ float scale_of(int byte) { return __builtin_bit_cast(float, (uint32_t)byte << 23); }
+
+// the largest over the 16 lanes of a row of the wave
+__device__ __forceinline__ uint32_t max16(uint32_t m) {
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, true));   // quad: 1 0 3 2
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));   // quad: 2 3 0 1
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, true));  // half row mirrored
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xf, 0xf, true));  // row mirrored
+  return m;
+}
+
+// One 128 x 128 tile a workgroup, read once: codes in blocks along the rows
+// and, transposed, along the columns, and partial column sums.  Thread t holds
+// columns 8 (t % 16) .. + 7 of rows 8 (t / 16) .. + 7 as they were stored: a
+// row's block is 16 lanes, and 8 rows of a column are 8 bytes of the
+// transposed codes, put together through LDS so that whole 128-byte lines are
+// written.
+template <typename E>
+__global__ __launch_bounds__(256, 4) void k_fp8_quant_tile(Fp8QuantArgs a) {
+  using X = Eight<E>;
+  __shared__ __attribute__((aligned(16))) uint8_t cols[128 * 128];
+  __shared__ __attribute__((aligned(16))) uint32_t red[4][X::NM * 16];
+  __shared__ uint32_t wave_max[4];
+  const int64_t k0 = (int64_t)blockIdx.x * 128, m0 = (int64_t)blockIdx.y * 128;
+  const int t = threadIdx.x, cl = t & 15, g = t >> 4, c0 = cl * 8, wave = t >> 6;
+  const int64_t rows = a.M - m0, width = a.K - k0;
+  const int64_t kp = fp8_kp(a.K), ksp = fp8_sp(a.K), mp = fp8_kp(a.M), msp = fp8_sp(a.M);
+  const int valid = width - c0 >= 8 ? 8 : width - c0 > 0 ? (int)(width - c0) : 0;
+  X x[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+  for (int i = 0; i < 8; ++i) {
+    const int r = g * 8 + i;
+    x[i].load((const E*)a.x + (m0 + r) * a.ld + k0 + c0, r < rows ? valid : 0);
+  }
+  if (a.slab) {
+    float* part = reinterpret_cast<float*>(cols);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
       float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s += v[i][j];
-      fr[rq * 128 + cq + j] = s;
+      for (int i = 0; i < 8; ++i) s += x[i].value(j);
+      part[g * 128 + c0 + j] = s;
     }
     __syncthreads();
     if (t < 128 && t < width) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) s += fr[w * 128 + t];
+      for (int i = 0; i < 16; ++i) s += part[i * 128 + t];
       a.slab[(int64_t)blockIdx.y * a.K + k0 + t] = s;
     }
     __syncthreads();
   }
-  uint32_t rowmax[16], colmax[4] = {0, 0, 0, 0};
+  // largest magnitudes of this thread's rows and columns; once more without what is not finite, where there is any
+  uint32_t rm[8], cm[X::NM];
+  auto largest = [&](auto f) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    uint32_t m = 0;
+    for (int k = 0; k < X::NM; ++k) cm[k] = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t b = finite_bits(v[i][j]);
-      m = max(m, b);
-      colmax[j] = max(colmax[j], b);
+    for (int i = 0; i < 8; ++i) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int k = 0; k < X::NM; ++k) {
+        const uint32_t q = f(x[i].mag(k));
+        m = X::larger(m, q);
+        cm[k] = X::larger(cm[k], q);
+      }
+      rm[i] = X::top(m);
     }
-    rowmax[i] = m;
+  };
+  largest([](uint32_t m) { return m; });
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) all = max(all, rm[i]);
+  if (__any(all >= X::kInf)) {
+    largest([](uint32_t m) { return X::finite(m); });
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) all = max(all, rm[i]);
   }
   int tile_byte = 0;
   if (a.tile) {
-    uint32_t m = max(max(colmax[0], colmax[1]), max(colmax[2], colmax[3]));
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-    if ((t & 63) == 0) tile_max[t >> 6] = m;
+    uint32_t m = max16(all);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+    if ((t & 63) == 0) wave_max[wave] = m;
     __syncthreads();
-    tile_byte = scale_byte(max(max(tile_max[0], tile_max[1]), max(tile_max[2], tile_max[3])));
+    tile_byte = scale_byte(X::bits(max(max(wave_max[0], wave_max[1]), max(wave_max[2], wave_max[3]))));
   }
   if (a.row_codes) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      uint32_t m = rowmax[i];
-      int byte = tile_byte;
-      if (!a.tile) {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-        byte = scale_byte(m);
-      }
-      const int r = rq * 16 + i;
-      if (r >= rows) continue;
-      const float inv = inverse_scale(byte);
-      *reinterpret_cast<uint32_t*>(a.row_codes + (m0 + r) * kp + k0 + cq) =
-          codes4(scaled(v[i][0], inv), scaled(v[i][1], inv), scaled(v[i][2], inv), scaled(v[i][3], inv));
-      if ((t & 31) == 0) {
+    for (int i = 0; i < 8; ++i) {
+      const int byte = a.tile ? tile_byte : scale_byte(X::bits(max16(rm[i])));
+      const int r = g * 8 + i;
+      if (r >= rows) continue;  // the same for the 16 lanes of a row
+      const float scale = scale_of(byte);
+      *reinterpret_cast<uint2*>(a.row_codes + (m0 + r) * kp + k0 + c0) = x[i].row_codes(scale);
+      if (cl == 0) {
         uint8_t* s = a.row_scales + (m0 + r) * ksp;
         s[blockIdx.x] = (uint8_t)byte;
         if (blockIdx.x == gridDim.x - 1)
@@ -184,32 +286,35 @@ __global__ __launch_bounds__(256) void k_fp8_quant_tile(Fp8QuantArgs a) {
   if (a.col_codes) {
     if (!a.tile) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) red[rq][cq + j] = colmax[j];
+      for (int k = 0; k < X::NM; ++k) {
+        cm[k] = X::larger(cm[k], (uint32_t)__shfl_xor((int)cm[k], 16));
+        cm[k] = X::larger(cm[k], (uint32_t)__shfl_xor((int)cm[k], 32));
+      }
+      if ((t & 63) < 16) {
+#pragma unroll
+        for (int k = 0; k < X::NM; ++k) red[wave][cl * X::NM + k] = cm[k];
+      }
       __syncthreads();
+#pragma unroll
+      for (int k = 0; k < X::NM; ++k) {
+        const int q = cl * X::NM + k;
+        cm[k] = X::larger(X::larger(red[0][q], red[1][q]), X::larger(red[2][q], red[3][q]));
+      }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      int byte = tile_byte;
-      const int c = cq + j;
-      if (!a.tile) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) m = max(m, red[w][c]);
-        byte = scale_byte(m);
-      }
-      const float inv = inverse_scale(byte);
-      uint32_t q[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        q[i] = codes4(scaled(v[4 * i][j], inv), scaled(v[4 * i + 1][j], inv), scaled(v[4 * i + 2][j], inv),
-                      scaled(v[4 * i + 3][j], inv));
-      // 16-byte piece rq of column c, pieces turned by the column so that writes and reads spread over the banks
-      *reinterpret_cast<uint4*>(cols + c * 128 + ((rq ^ (c >> 2)) & 7) * 16) = make_uint4(q[0], q[1], q[2], q[3]);
-      if (rq == 0 && c < width) {
+    for (int j = 0; j < 8; ++j) {
+      const int byte = a.tile ? tile_byte
+                              : scale_byte(X::bits(X::WIDE ? cm[X::WIDE ? j : 0] : cm[j / 2 % X::NM] >> (16 * (j & 1)) & 0xffffu));
+      const float scale = scale_of(byte);
+      const int c = c0 + j;
+      // 16-byte piece g / 2 of column c, pieces turned by the thread so that writes spread over the banks
+      *reinterpret_cast<uint2*>(cols + c * 128 + ((g >> 1 ^ cl) & 7) * 16 + (g & 1) * 8) =
+          make_uint2(X::col_codes(x, j, scale), X::col_codes(x + 4, j, scale));
+      if (g == 0 && c < width) {
         uint8_t* s = a.col_scales + (k0 + c) * msp;
         s[blockIdx.y] = (uint8_t)byte;
         if (blockIdx.y == gridDim.y - 1)
-          for (int64_t i = gridDim.y; i < msp; ++i) s[i] = 127;
+          for (int64_t q = gridDim.y; q < msp; ++q) s[q] = 127;
       }
     }
     __syncthreads();
@@ -218,23 +323,9 @@ __global__ __launch_bounds__(256) void k_fp8_quant_tile(Fp8QuantArgs a) {
       const int p = i * 256 + t, c = p >> 3, w = p & 7;
       if (c < width)
         *reinterpret_cast<uint4*>(a.col_codes + (k0 + c) * mp + m0 + w * 16) =
-            *reinterpret_cast<const uint4*>(cols + c * 128 + ((w ^ (c >> 2)) & 7) * 16);
+            *reinterpret_cast<const uint4*>(cols + c * 128 + ((w ^ c >> 3) & 7) * 16);
     }
   }
-}
-
-// out[c] = sum of the slab rows in order: 64 columns a workgroup, 4 waves share the rows
-__global__ __launch_bounds__(256) void k_fp8_colsum(const float* __restrict__ slab, int64_t rows, int64_t K,
-                                                    float* __restrict__ out) {
-  __shared__ float red[4][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-  float s = 0.f;
-  if (c < K)
-    for (int64_t r = w; r < rows; r += 4) s += slab[r * K + c];
-  red[w][lane] = s;
-  __syncthreads();
-  if (w == 0 && c < K) out[c] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
 
 // ---------------------------------------------------------------- product
@@ -581,54 +672,99 @@ __global__ __launch_bounds__(256) void k_fp8_join(Fp8GemmArgs g) {
   store4((C*)g.c + m * g.N + n, g.N - n, s + bias4(g.bias, n, g.N));
 }
 
-// Up to 16 MT rows of a: the bytes of b are the cost, so no LDS staging.  A
-// workgroup takes 16 rows of b, its 8 waves share the blocks of K and join
-// their sums through LDS in order.
-template <int MT, typename C>
+// Up to 16 MT rows of a: the bytes of b are the cost, so they go straight to
+// registers, three blocks ahead.  A workgroup takes 16 NT rows of b; its 8
+// waves share the blocks of K and join their sums through LDS in order.  Two
+// tiles of b a wave halve the reads of a, which come from the L2 for every
+// workgroup.
+template <int MT, int NT, typename C>
 __global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
-  __shared__ f32x4 part[8][MT][64];
+  using F = Frag<std::is_same<C, float>::value>;
+  constexpr int AHEAD = 3;
+  __shared__ f32x4 part[8][NT * MT][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 15, fg = lane >> 4;
   const int64_t kp = fp8_kp(g.K), sp = fp8_sp(g.K);
-  const int nb = (int)(kp / 128);
-  const int n0 = blockIdx.x * 16;
-  const int64_t brow = min(n0 + fr, g.N - 1);
-  const uint8_t* pb = g.b + brow * kp + fg * 32;
-  const uint8_t* psb = g.sb + brow * sp;
-  const uint8_t *pa[MT], *psa[MT];
-  f32x4 acc[MT];
+  const int nb = (int)(kp / 128), b0 = (int)((int64_t)nb * w / 8), b1 = (int)((int64_t)nb * (w + 1) / 8);
+  const int n0 = blockIdx.x * 16 * NT;
+  const uint8_t *pa[MT], *psa[MT], *pb[NT], *psb[NT];
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int64_t r = min(n0 + j * 16 + fr, g.N - 1);
+    pb[j] = g.b + r * kp + fg * 32;
+    psb[j] = g.sb + r * sp;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int64_t r = min(i * 16 + fr, g.M - 1);
     pa[i] = g.a + r * kp + fg * 32;
     psa[i] = g.sa + r * sp;
-    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  using F = Frag<std::is_same<C, float>::value>;
-  auto load = [](const uint8_t* p, uint32_t byte) { return F(codes32(p, p + 16), byte); };
-  for (int kb = w; kb < nb; kb += 8) {
-    const F fb = load(pb + (int64_t)kb * 128, psb[kb]);
+  i32x8 va[AHEAD][MT], vb[AHEAD][NT];
+  uint8_t ea[AHEAD][MT], eb[AHEAD][NT];
+  auto load = [&](int at, int kb) {
+    kb = min(kb, nb - 1);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i] = mfma_blocks(fb, load(pa[i] + (int64_t)kb * 128, psa[i][kb]), acc[i]);
+    for (int j = 0; j < NT; ++j) {
+      vb[at][j] = codes32(pb[j] + (int64_t)kb * 128, pb[j] + (int64_t)kb * 128 + 16);
+      eb[at][j] = psb[j][kb];
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      va[at][i] = codes32(pa[i] + (int64_t)kb * 128, pa[i] + (int64_t)kb * 128 + 16);
+      ea[at][i] = psa[i][kb];
+    }
+  };
+  if (b0 < b1) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) load(u, b0 + u);
+  }
+  for (int kb = b0; kb < b1; kb += AHEAD) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (kb + u >= b1) break;
+      F b[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) b[j] = F(vb[u][j], eb[u][j]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const F a(va[u][i], ea[u][i]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[j][i] = mfma_blocks(b[j], a, acc[j][i]);
+      }
+      if (kb + u + AHEAD < b1) load(u, kb + u + AHEAD);
+    }
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i) part[w][i][lane] = acc[i];
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) part[w][j * MT + i][lane] = acc[j][i];
   __syncthreads();
-  if (w < MT) {
+  if (w < NT * MT) {
     f32x4 s = part[0][w][lane];
 #pragma unroll
     for (int k = 1; k < 8; ++k) s += part[k][w][lane];
-    const int m = w * 16 + fr, n = n0 + fg * 4;
+    const int m = w % MT * 16 + fr, n = n0 + w / MT * 16 + fg * 4;
     if (m < g.M && n < g.N) store4((C*)g.c + (int64_t)m * g.N + n, g.N - n, s + bias4(g.bias, n, g.N));
   }
+}
+
+template <int NT, typename C>
+void skinny(const Fp8GemmArgs& g, hipStream_t s) {
+  const dim3 grid((g.N + 16 * NT - 1) / (16 * NT));
+  if (g.M <= 16) hipLaunchKernelGGL((k_fp8_skinny<1, NT, C>), grid, dim3(512), 0, s, g);
+  else if (g.M <= 32) hipLaunchKernelGGL((k_fp8_skinny<2, NT, C>), grid, dim3(512), 0, s, g);
+  else if (g.M <= 48) hipLaunchKernelGGL((k_fp8_skinny<3, NT, C>), grid, dim3(512), 0, s, g);
+  else hipLaunchKernelGGL((k_fp8_skinny<4, NT, C>), grid, dim3(512), 0, s, g);
 }
 
 template <typename C>
 void gemm(const Fp8GemmArgs& g, hipStream_t s) {
   if (g.M <= 64) {
-    const dim3 grid((g.N + 15) / 16);
-    if (g.M <= 16) hipLaunchKernelGGL((k_fp8_skinny<1, C>), grid, dim3(512), 0, s, g);
-    else if (g.M <= 32) hipLaunchKernelGGL((k_fp8_skinny<2, C>), grid, dim3(512), 0, s, g);
-    else hipLaunchKernelGGL((k_fp8_skinny<4, C>), grid, dim3(512), 0, s, g);
+    if (g.M > 16 && g.N >= 4096) skinny<2, C>(g, s);
+    else skinny<1, C>(g, s);
     return;
   }
   auto tiles = [&](int bm, int bn) { return dim3((unsigned)((int64_t)((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn)), 1, g.ksplit); };
@@ -674,7 +810,7 @@ void quant(const Fp8QuantArgs& a, hipStream_t s) {
   const int64_t mb = (a.M + 127) / 128;
   hipLaunchKernelGGL(k_fp8_quant_tile<E>, dim3((unsigned)kb, (unsigned)mb), dim3(256), 0, s, a);
   if (a.colsum)
-    hipLaunchKernelGGL(k_fp8_colsum, dim3((unsigned)((a.K + 63) / 64)), dim3(256), 0, s, a.slab, mb, a.K, a.colsum);
+    launch_block_cols(a.slab, mb, a.K, &a.colsum, 1, a.K, s);
 }
 }  // namespace
 

@@ -177,7 +177,7 @@ __device__ __forceinline__ void norm_back(float g[C][8], float n[C][8], const in
 
 // Column sums (weights, biases, channel gate) stay in registers over the rows
 // a group walks, are added over the groups of a workgroup in order and leave
-// as one slab row; k_residual_cols adds the slab rows in order: no atomics, the
+// as one slab row; k_block_cols adds the slab rows in order: no atomics, the
 // same bits every time.
 template <int TR, int TT, int L, int C>
 __global__ __launch_bounds__(L < 256 ? 256 : L) void k_residual_bwd(ResidualArgs a) {
@@ -333,31 +333,30 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_residual_bwd(ResidualArgs
 struct ColOut {
   float* p[5];
 };
-// out[v][c] = sum of the slab rows, in order: 64 columns a workgroup, 4 waves
-// share the rows
-__global__ __launch_bounds__(256) void k_residual_cols(const float* __restrict__ slab, int rows, int nvec, int D, ColOut o) {
-  __shared__ float red[4][64];
+// out[v][c] = sum over the slab's rows, in an order of their number alone: 64
+// columns a workgroup, 16 waves take every 16th row, eight loads in flight.
+__global__ __launch_bounds__(1024) void k_block_cols(const float* __restrict__ slab, int64_t rows, int64_t W, int64_t D,
+                                                     ColOut o) {
+  __shared__ float red[16][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t W = (int64_t)nvec * D;
   const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+  float s[8] = {};
   if (c < W) {
-    int r = w;
-    for (; r + 12 < rows; r += 16) {
-      s0 += slab[(int64_t)r * W + c];
-      s1 += slab[(int64_t)(r + 4) * W + c];
-      s2 += slab[(int64_t)(r + 8) * W + c];
-      s3 += slab[(int64_t)(r + 12) * W + c];
-    }
-    for (; r < rows; r += 4) s0 += slab[(int64_t)r * W + c];
+    int64_t r = w;
+    for (; r + 112 < rows; r += 128)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += slab[(r + 16 * i) * W + c];
+    for (; r < rows; r += 16) s[0] += slab[r * W + c];
   }
-  red[w][lane] = (s0 + s1) + (s2 + s3);
+  red[w][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   __syncthreads();
   if (w == 0 && c < W) {
-    const float s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) q += red[i][lane];
     const int v = (int)(c / D);
     float* p = v == 0 ? o.p[0] : v == 1 ? o.p[1] : v == 2 ? o.p[2] : v == 3 ? o.p[3] : o.p[4];
-    p[c - (int64_t)v * D] = s;
+    p[c - (int64_t)v * D] = q;
   }
 }
 
@@ -432,15 +431,20 @@ void launch_residual_bwd(const ResidualArgs& a, hipStream_t s) {
   });
   const int nvec = residual_nvec(a);
   if (!nvec) return;
-  ColOut o{};
+  float* out[5];
   int v = 0;
-  if (a.dpre_w) o.p[v++] = a.dpre_w;
-  if (a.dpre_b) o.p[v++] = a.dpre_b;
-  if (a.gate_kind == kGateChannel && a.dgate) o.p[v++] = (float*)a.dgate;
-  if (a.dpost_w) o.p[v++] = a.dpost_w;
-  if (a.dpost_b) o.p[v++] = a.dpost_b;
-  const int64_t W = (int64_t)nvec * a.D;
-  hipLaunchKernelGGL(k_residual_cols, dim3((unsigned)((W + 63) / 64)), dim3(256), 0, s, a.slab, grid, nvec, a.D, o);
+  if (a.dpre_w) out[v++] = a.dpre_w;
+  if (a.dpre_b) out[v++] = a.dpre_b;
+  if (a.gate_kind == kGateChannel && a.dgate) out[v++] = (float*)a.dgate;
+  if (a.dpost_w) out[v++] = a.dpost_w;
+  if (a.dpost_b) out[v++] = a.dpost_b;
+  launch_block_cols(a.slab, grid, (int64_t)nvec * a.D, out, nvec, a.D, s);
+}
+
+void launch_block_cols(const float* slab, int64_t rows, int64_t W, float* const* out, int nout, int64_t D, hipStream_t s) {
+  ColOut o{};
+  for (int i = 0; i < nout; ++i) o.p[i] = out[i];
+  hipLaunchKernelGGL(k_block_cols, dim3((unsigned)((W + 63) / 64)), dim3(1024), 0, s, slab, rows, W, D, o);
 }
 
 void launch_dropout(const void* x, void* y, int64_t n, BlockType t, const MaskArgs& m, hipStream_t s) {

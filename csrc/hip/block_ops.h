@@ -30,6 +30,9 @@ struct MaskArgs {
 // y[i] = keep(i) ? x[i] * up : 0, n elements of one type
 void launch_dropout(const void* x, void* y, int64_t n, BlockType t, const MaskArgs& m, hipStream_t s);
 
+// out[v][c] = sum of slab[r][v D + c] over rows, v < nout <= 5, W = nout D
+void launch_block_cols(const float* slab, int64_t rows, int64_t W, float* const* out, int nout, int64_t D, hipStream_t s);
+
 // ---------------------------------------------------------------- gated residual norm
 enum NormKind : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
 enum GateKind : int { kGateNone = 0, kGateChannel = 1, kGateRow = 2, kGateFull = 3 };
