@@ -104,21 +104,24 @@ struct Eight {
   static constexpr int NM = WIDE ? 8 : 4;  // dwords
   typedef uint32_t dwords __attribute__((ext_vector_type(NM)));
   dwords d;
+  __device__ __forceinline__ void load(const E* p) { d = __builtin_bit_cast(dwords, *reinterpret_cast<const vec8*>(p)); }
+  // `valid` values of them; the others come from the first address and count as 0
   __device__ __forceinline__ void load(const E* p, int valid) {
-    if (valid >= 8) {
-      d = __builtin_bit_cast(dwords, *reinterpret_cast<const vec8*>(p));
-    } else {
 #pragma unroll
-      for (int k = 0; k < NM; ++k) {
-        if constexpr (WIDE) {
-          d[k] = k < valid ? __builtin_bit_cast(uint32_t, p[k]) : 0u;
-        } else {
-          const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
-          const uint32_t lo = 2 * k < valid ? q[2 * k] : 0u, hi = 2 * k + 1 < valid ? q[2 * k + 1] : 0u;
-          d[k] = lo | hi << 16;
-        }
+    for (int k = 0; k < NM; ++k) {
+      if constexpr (WIDE) {
+        const uint32_t x = __builtin_bit_cast(uint32_t, p[k < valid ? k : 0]);
+        d[k] = k < valid ? x : 0u;
+      } else {
+        const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+        const uint32_t lo = q[2 * k < valid ? 2 * k : 0], hi = q[2 * k + 1 < valid ? 2 * k + 1 : 0];
+        d[k] = (2 * k < valid ? lo : 0u) | (2 * k + 1 < valid ? hi << 16 : 0u);
       }
     }
+  }
+  __device__ __forceinline__ void only_if(bool keep) {
+#pragma unroll
+    for (int k = 0; k < NM; ++k) d[k] = keep ? d[k] : 0u;
   }
   __device__ __forceinline__ float value(int j) const {
     if constexpr (WIDE) return __builtin_bit_cast(float, (uint32_t)d[j]);
@@ -197,7 +200,7 @@ __device__ __forceinline__ uint32_t max16(uint32_t m) {
 // transposed codes, put together through LDS so that whole 128-byte lines are
 // written.
 template <typename E>
-__global__ __launch_bounds__(256, 4) void k_fp8_quant_tile(Fp8QuantArgs a) {
+__global__ __launch_bounds__(256, sizeof(E) == 4 ? 3 : 4) void k_fp8_quant_tile(Fp8QuantArgs a) {
   using X = Eight<E>;
   __shared__ __attribute__((aligned(16))) uint8_t cols[128 * 128];
   __shared__ __attribute__((aligned(16))) uint32_t red[4][X::NM * 16];
@@ -208,10 +211,18 @@ __global__ __launch_bounds__(256, 4) void k_fp8_quant_tile(Fp8QuantArgs a) {
   const int64_t kp = fp8_kp(a.K), ksp = fp8_sp(a.K), mp = fp8_kp(a.M), msp = fp8_sp(a.M);
   const int valid = width - c0 >= 8 ? 8 : width - c0 > 0 ? (int)(width - c0) : 0;
   X x[8];
+  // loads without a branch between them; rows and columns past the end read the last row and the first column
+  const E* from = (const E*)a.x + m0 * a.ld + k0 + (valid ? c0 : 0);
+  if (width >= 128 || width % 8 == 0) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = g * 8 + i;
-    x[i].load((const E*)a.x + (m0 + r) * a.ld + k0 + c0, r < rows ? valid : 0);
+    for (int i = 0; i < 8; ++i) x[i].load(from + min((int64_t)(g * 8 + i), rows - 1) * a.ld);
+    if (rows < 128 || width < 128) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i].only_if(g * 8 + i < rows && valid);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i].load(from + min((int64_t)(g * 8 + i), rows - 1) * a.ld, g * 8 + i < rows ? valid : 0);
   }
   if (a.slab) {
     float* part = reinterpret_cast<float*>(cols);
@@ -705,7 +716,6 @@ __global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
   i32x8 va[AHEAD][MT], vb[AHEAD][NT];
   uint8_t ea[AHEAD][MT], eb[AHEAD][NT];
   auto load = [&](int at, int kb) {
-    kb = min(kb, nb - 1);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
       vb[at][j] = codes32(pb[j] + (int64_t)kb * 128, pb[j] + (int64_t)kb * 128 + 16);
@@ -717,10 +727,9 @@ __global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
       ea[at][i] = psa[i][kb];
     }
   };
-  if (b0 < b1) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) load(u, b0 + u);
-  }
+  for (int u = 0; u < AHEAD; ++u)
+    if (b0 + u < b1) load(u, b0 + u);
   for (int kb = b0; kb < b1; kb += AHEAD) {
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
