@@ -73,6 +73,12 @@ int residual_slab_rows(int64_t M, int D);
 constexpr int kResidualMaxD = 16384;
 void launch_residual_fwd(const ResidualArgs& a, hipStream_t s);
 void launch_residual_bwd(const ResidualArgs& a, hipStream_t s);
+// its kernel by types (stream and, where it differs, the rest)
+void launch_residual_bwd_f32(const ResidualArgs& a, int grid, hipStream_t s);
+void launch_residual_bwd_bf16(const ResidualArgs& a, int grid, hipStream_t s);
+void launch_residual_bwd_f16(const ResidualArgs& a, int grid, hipStream_t s);
+void launch_residual_bwd_f32_bf16(const ResidualArgs& a, int grid, hipStream_t s);
+void launch_residual_bwd_f32_f16(const ResidualArgs& a, int grid, hipStream_t s);
 
 // ---------------------------------------------------------------- 8-bit blocks
 // A matrix [rows, K] held in e4m3 with one power-of-two scale for each block
