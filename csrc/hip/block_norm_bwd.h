@@ -12,16 +12,15 @@ namespace {
 template <int L, int C, bool N>
 __device__ __forceinline__ void norm_back(float g[C][8], const float n[C][8], const Columns<L, C, N>& at, int kind, float inv,
                                           float* red) {
-  float sgn = 0.f, sg = 0.f;
+  float s[2] = {0.f, 0.f};  // of g n and, for the layer norm, of g
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      sgn += at.counts(c, j) ? g[c][j] * n[c][j] : 0.f;
-      if (kind == kNormLayer) sg += at.counts(c, j) ? g[c][j] : 0.f;
-    }
-  sgn = row_sum<L>(sgn, red) / (float)at.width;
-  if (kind == kNormLayer) sg = row_sum<L>(sg, red + 16) / (float)at.width;
+  for (int c = 0; c < C; ++c) {
+    s[0] += at.sum(c, [&](int j) { return g[c][j] * n[c][j]; });
+    if (kind == kNormLayer) s[1] += at.sum(c, [&](int j) { return g[c][j]; });
+  }
+  if (kind == kNormLayer) row_sums<L>(s, red);
+  else s[0] = row_sum<L>(s[0], red);
+  const float sgn = s[0] * at.per, sg = s[1] * at.per;
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -35,8 +34,10 @@ __device__ __forceinline__ void norm_back(float g[C][8], const float n[C][8], co
 //
 // LAYER: either norm has a bias, GATE: the gate is one of channels: which sums
 // there are to hold.  With those that are not needed held as well the kernel
-// took 180 registers a lane, one workgroup a CU, and twice the time.
-template <int TR, int TT, int L, int C, bool N, bool LAYER, bool GATE>
+// took 180 registers a lane, one workgroup a CU, and twice the time.  ALL: both
+// norms are there, all of dr, dh, dx and dy wanted, as in training: the
+// conditions on them otherwise fill the scalar registers.
+template <int TR, int TT, int L, int C, bool N, bool LAYER, bool GATE, bool ALL>
 __global__ __launch_bounds__(L < 256 ? 256 : L, L < 512 ? 2 : L == 512 && !LAYER ? 4 : 1) void k_residual_bwd(ResidualArgs a) {
   using R = typename BlockElem<TR>::type;
   using E = typename BlockElem<TT>::type;
@@ -56,23 +57,35 @@ __global__ __launch_bounds__(L < 256 ? 256 : L, L < 512 ? 2 : L == 512 && !LAYER
       if (LAYER) s_preb[c][j] = s_postb[c][j] = 0.f;
       if (GATE) s_gate[c][j] = 0.f;
     }
-  const bool pre = a.pre && a.dh;
-  int it = 0;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + grp; row < a.M; row += (int64_t)gridDim.x * kRows, it ^= 1) {
-    float* rd = red[it];  // two sets in turn: a wave may be one row ahead of another, never two
+  const bool pre = ALL || (a.pre && a.dh), post = ALL || a.post, has_dr = ALL || a.dr;
+  const int pre_kind = LAYER ? a.pre : kNormRms, post_kind = LAYER ? a.post : kNormRms;  // where there is one
+  struct Raw {
     Vec8<E> y[C], dh[C], gf[C];
     Vec8<R> x[C], dr[C];
+    float4 st;
+  };
+  auto fetch = [&](Raw& v, int64_t row) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      y[c] = at.load(c, (const E*)a.y + row * a.ldy);
+      v.y[c] = at.load(c, (const E*)a.y + row * a.ldy);
       if (pre) {
-        x[c] = at.load(c, (const R*)a.x + row * a.ldx);
-        dh[c] = at.load(c, (const E*)a.dh + row * a.lddh);
+        v.x[c] = at.load(c, (const R*)a.x + row * a.ldx);
+        v.dh[c] = at.load(c, (const E*)a.dh + row * a.lddh);
       }
-      if (a.dr) dr[c] = at.load(c, (const R*)a.dr + row * a.lddr);
-      if (!GATE && a.gate_kind == kGateFull) gf[c] = at.load(c, (const E*)a.gate + row * a.ldg);
+      if (has_dr) v.dr[c] = at.load(c, (const R*)a.dr + row * a.lddr);
+      if (!GATE && a.gate_kind == kGateFull) v.gf[c] = at.load(c, (const E*)a.gate + row * a.ldg);
     }
-    const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
+    v.st = reinterpret_cast<const float4*>(a.stats)[row];
+  };
+  const int64_t first = (int64_t)blockIdx.x * kRows + grp, step = (int64_t)gridDim.x * kRows;
+  int it = 0;
+  for (int64_t row = first; row < a.M; row += step, it ^= 1) {
+    float* rd = red[it];  // two sets in turn: a wave may be one row ahead of another, never two
+    Raw raw;
+    fetch(raw, row);
+    const auto &y = raw.y, &dh = raw.dh, &gf = raw.gf;
+    const auto &x = raw.x, &dr = raw.dr;
+    const float4 st = raw.st;
     float grow = 1.f;
     if (!GATE && a.gate_kind == kGateRow) {
       grow = ((const float*)a.gate)[row];
@@ -86,11 +99,11 @@ __global__ __launch_bounds__(L < 256 ? 256 : L, L < 512 ? 2 : L == 512 && !LAYER
       keep[c] = a.mask.thr ? keep8(row * a.D + at.col[c], sd.seed, sd.offset, a.mask.thr) : 0xffu;
 #pragma unroll
       for (int j = 0; j < 8; ++j) un[c][j] = d[c][j] = (float)y[c][j];
-      if (a.post) {
+      if (post) {
         const Vec8<float> w = at.load(c, a.post_w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          un[c][j] = (un[c][j] - st.x) * st.y;
+          un[c][j] = LAYER ? (un[c][j] - st.x) * st.y : un[c][j] * st.y;
           d[c][j] = un[c][j] * w[j];
         }
         if (LAYER && a.post_b) {
@@ -122,13 +135,13 @@ __global__ __launch_bounds__(L < 256 ? 256 : L, L < 512 ? 2 : L == 512 && !LAYER
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float r = a.x_scale * (float)x[c][j] + a.y_scale * (gv[c][j] * d[c][j]), g = (float)dh[c][j];
-          n[c][j] = (r - st.z) * st.w;
+          n[c][j] = LAYER ? (r - st.z) * st.w : r * st.w;
           s_prew[c][j] += g * n[c][j];
           if (LAYER) s_preb[c][j] += g;
           t[c][j] = g * w[j];
         }
       }
-      norm_back<L, C, N>(t, n, at, a.pre, st.w, rd);
+      norm_back<L, C, N>(t, n, at, pre_kind, st.w, rd);
     } else {
 #pragma unroll
       for (int c = 0; c < C; ++c)
@@ -139,11 +152,11 @@ __global__ __launch_bounds__(L < 256 ? 256 : L, L < 512 ? 2 : L == 512 && !LAYER
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       float g[8];
-      if (a.dr) {
+      if (has_dr) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) t[c][j] += (float)dr[c][j];
       }
-      if (a.dx) {
+      if (ALL || a.dx) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] = a.x_scale * t[c][j];
         at.store(c, (R*)a.dx + row * a.D, g);
@@ -155,13 +168,13 @@ __global__ __launch_bounds__(L < 256 ? 256 : L, L < 512 ? 2 : L == 512 && !LAYER
         g[j] = t[c][j] * d[c][j];
         if (a.sigmoid && (GATE || a.gate_kind != kGateRow)) g[j] *= gv[c][j] * (1.f - gv[c][j]);
         if (GATE) s_gate[c][j] += g[j];
-        gdot += at.counts(c, j) ? g[j] : 0.f;
         t[c][j] = (keep[c] >> j & 1) ? t[c][j] * gv[c][j] * a.mask.up : 0.f;
         s_postw[c][j] += t[c][j] * un[c][j];
         if (LAYER) s_postb[c][j] += t[c][j];
       }
+      if (!GATE && a.gate_kind == kGateRow) gdot += at.sum(c, [&](int j) { return g[j]; });
       if (!GATE && a.gate_kind == kGateFull && a.dgate) at.store(c, (E*)a.dgate + row * a.D, g);
-      if (a.post) {
+      if (post) {
         const Vec8<float> w = at.load(c, a.post_w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) t[c][j] *= w[j];
@@ -171,8 +184,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L, L < 512 ? 2 : L == 512 && !LAYER
       gdot = row_sum<L>(gdot, rd + 32);
       if (lane == 0) ((float*)a.dgate)[row] = a.sigmoid ? gdot * grow * (1.f - grow) : gdot;
     }
-    if (a.dy) {
-      if (a.post) norm_back<L, C, N>(t, un, at, a.post, st.y, rd + 64);
+    if (ALL || a.dy) {
+      if (post) norm_back<L, C, N>(t, un, at, post_kind, st.y, rd + 64);
 #pragma unroll
       for (int c = 0; c < C; ++c) at.store(c, (E*)a.dy + row * a.D, t[c]);
     }
@@ -211,14 +224,20 @@ __global__ __launch_bounds__(L < 256 ? 256 : L, L < 512 ? 2 : L == 512 && !LAYER
 template <int TR, int TT>
 void residual_bwd(const ResidualArgs& a, int grid, hipStream_t s) {
   const bool layer = a.post == kNormLayer || a.pre == kNormLayer, gate = a.gate_kind == kGateChannel;
+  const bool all = a.post && a.pre && a.dr && a.dh && a.dx && a.dy;
   by_width(a.D, [&](auto l, auto c, auto n) {
     constexpr int L = decltype(l)::value, C = decltype(c)::value;
     constexpr bool N = decltype(n)::value;
     const dim3 g(grid), b(L < 256 ? 256 : L);
-    if (layer && gate) hipLaunchKernelGGL((k_residual_bwd<TR, TT, L, C, N, true, true>), g, b, 0, s, a);
-    else if (layer) hipLaunchKernelGGL((k_residual_bwd<TR, TT, L, C, N, true, false>), g, b, 0, s, a);
-    else if (gate) hipLaunchKernelGGL((k_residual_bwd<TR, TT, L, C, N, false, true>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((k_residual_bwd<TR, TT, L, C, N, false, false>), g, b, 0, s, a);
+    auto go = [&](auto layer_t, auto gate_t) {
+      constexpr bool LA = decltype(layer_t)::value, GA = decltype(gate_t)::value;
+      if (all) hipLaunchKernelGGL((k_residual_bwd<TR, TT, L, C, N, LA, GA, true>), g, b, 0, s, a);
+      else hipLaunchKernelGGL((k_residual_bwd<TR, TT, L, C, N, LA, GA, false>), g, b, 0, s, a);
+    };
+    if (layer && gate) go(std::true_type{}, std::true_type{});
+    else if (layer) go(std::true_type{}, std::false_type{});
+    else if (gate) go(std::false_type{}, std::true_type{});
+    else go(std::false_type{}, std::false_type{});
   });
 }
 

@@ -15,20 +15,50 @@ template <typename E>
 using Vec8 = E __attribute__((ext_vector_type(8), aligned(sizeof(E))));
 
 
-// sum over the L threads that share a row; red: LDS of one float a wave, its
-// own for each call of a row (so one barrier a call suffices)
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// sum over 16 lanes, in each of them, and over the wave: lane moves within the
+// vector pipe (a shuffle through LDS costs ten times the latency)
+__device__ __forceinline__ float sum16(float v) {
+  v += dpp<0xB1>(v);   // quad: 1 0 3 2
+  v += dpp<0x4E>(v);   // quad: 2 3 0 1
+  v += dpp<0x141>(v);  // half row mirrored
+  v += dpp<0x140>(v);  // row mirrored
+  return v;
+}
+__device__ __forceinline__ float sum64(float v) {
+  const int s = __builtin_bit_cast(int, sum16(v));
+  auto lane = [&](int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(s, l)); };
+  return (lane(0) + lane(16)) + (lane(32) + lane(48));
+}
+
+// sums of K values over the L threads that share a row; red: LDS of K floats a
+// wave, its own for each call of a row (so one barrier a call suffices)
+template <int L, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float* red) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = L == 16 ? sum16(v[k]) : sum64(v[k]);
+  if constexpr (L > 64) {
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[(threadIdx.x >> 6) * K + k] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < L / 64; ++w) v[k] += red[w * K + k];
+    }
+  }
+}
 template <int L>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-#pragma unroll
-  for (int o = 1; o < (L < 64 ? L : 64); o <<= 1) v += __shfl_xor(v, o);
-  if constexpr (L > 64) {
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0.f;
-#pragma unroll
-    for (int w = 0; w < L / 64; ++w) v += red[w];
-  }
-  return v;
+  float a[1] = {v};
+  row_sums<L>(a, red);
+  return a[0];
 }
 
 __device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
@@ -56,7 +86,8 @@ __device__ __forceinline__ void keep_seed(const MaskArgs& m, const Seed& s) {
 template <int L, int C, bool NARROW>
 struct Columns {
   int col[C], skip[C], width;
-  __device__ __forceinline__ Columns(int lane, int D) : width(D) {
+  float per;  // 1 / width
+  __device__ __forceinline__ Columns(int lane, int D) : width(D), per(1.f / (float)D) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int at = (c * L + lane) * 8;
@@ -66,6 +97,24 @@ struct Columns {
   }
   __device__ __forceinline__ bool any(int c) const { return skip[c] < 8; }
   __device__ __forceinline__ bool counts(int c, int j) const { return NARROW ? skip[c] == 0 && j < width : j >= skip[c]; }
+  // sum of f(j) over the columns of chunk c that count; the rare chunk with others takes a branch of its own
+  template <typename F>
+  __device__ __forceinline__ float sum(int c, F f) const {
+    float s = 0.f;
+    if (NARROW) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += counts(c, j) ? f(j) : 0.f;
+      return s;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += f(j);
+    if (skip[c]) {
+      s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += j >= skip[c] ? f(j) : 0.f;
+    }
+    return s;
+  }
   template <typename E>
   __device__ __forceinline__ Vec8<E> load(int c, const E* row) const {
     Vec8<E> v;
@@ -100,10 +149,8 @@ __device__ __forceinline__ float2 normalise(float v[C][8], const Columns<L, C, N
   if (kind == kNormLayer) {
     float s = 0.f;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s += at.counts(c, j) ? v[c][j] : 0.f;
-    mean = row_sum<L>(s, red) / (float)at.width;
+    for (int c = 0; c < C; ++c) s += at.sum(c, [&](int j) { return v[c][j]; });
+    mean = row_sum<L>(s, red) * at.per;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -111,10 +158,8 @@ __device__ __forceinline__ float2 normalise(float v[C][8], const Columns<L, C, N
   }
   float q = 0.f;
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) q += at.counts(c, j) ? v[c][j] * v[c][j] : 0.f;
-  const float inv = 1.f / sqrtf(row_sum<L>(q, red + 16) / (float)at.width + eps);
+  for (int c = 0; c < C; ++c) q += at.sum(c, [&](int j) { return v[c][j] * v[c][j]; });
+  const float inv = 1.f / sqrtf(row_sum<L>(q, red + 16) * at.per + eps);
 #pragma unroll
   for (int c = 0; c < C; ++c)
 #pragma unroll
