@@ -327,17 +327,29 @@ void fp8_dims(int64_t a, int64_t b) {
   BK_CHECK(a <= kFp8MaxDim && b <= kFp8MaxDim, "fp8: at most ", kFp8MaxDim, " rows or columns");
 }
 
-// codes and exponent bytes of a [rows, K] matrix in one allocation
+// codes and exponent bytes of a [rows, K] matrix, in a part of an allocation
 struct Fp8Buf {
-  Tensor mem;
+  uint8_t* codes = nullptr;
   int64_t rows = 0, K = 0;
-  uint8_t* codes() const { return mem.data_ptr<uint8_t>(); }
-  uint8_t* scales() const { return codes() + rows * fp8_kp(K); }
+  uint8_t* scales() const { return codes + rows * fp8_kp(K); }
+  static int64_t bytes(int64_t rows, int64_t K) { return (rows * (fp8_kp(K) + fp8_sp(K)) + 255) / 256 * 256; }
 };
-Fp8Buf fp8_buf(Tensor mem, int64_t rows, int64_t K) { return {mem, rows, K}; }
-Fp8Buf fp8_new(int64_t rows, int64_t K, const Tensor& like) {
-  return {torch::empty({rows * (fp8_kp(K) + fp8_sp(K))}, like.options().dtype(torch::kUInt8)), rows, K};
-}
+// parts of one allocation, each at a multiple of 256 bytes
+class Parts {
+ public:
+  int64_t add(int64_t bytes) {
+    const int64_t at = size_;
+    size_ += (bytes + 255) / 256 * 256;
+    return at;
+  }
+  void allocate(const Tensor& like) { mem = torch::empty({size_}, like.options().dtype(torch::kUInt8)); }
+  uint8_t* at(int64_t offset) const { return mem.data_ptr<uint8_t>() + offset; }
+  Fp8Buf blocks(int64_t offset, int64_t rows, int64_t K) const { return {at(offset), rows, K}; }
+  Tensor mem;
+
+ private:
+  int64_t size_ = 0;
+};
 
 Fp8QuantArgs quant_args(const Tensor& x, int64_t M, int64_t K, bool tile) {
   Fp8QuantArgs q;
@@ -350,8 +362,8 @@ Fp8QuantArgs quant_args(const Tensor& x, int64_t M, int64_t K, bool tile) {
   return q;
 }
 
-void fp8_product(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t* sb, int64_t M, int64_t N,
-                 int64_t K, const float* bias, const Tensor& c) {
+Fp8GemmArgs gemm_args(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const uint8_t* sb, int64_t M, int64_t N,
+                      int64_t K, const float* bias, const Tensor& c) {
   Fp8GemmArgs g;
   g.a = a;
   g.sa = sa;
@@ -363,17 +375,20 @@ void fp8_product(const uint8_t* a, const uint8_t* sa, const uint8_t* b, const ui
   g.bias = bias;
   g.c = c.data_ptr();
   g.ct = block_type(c, "the result");
-  g.ksplit = fp8_gemm_ksplit(g.M, g.N, K);
+  return g;
+}
+Fp8GemmArgs gemm_args(const Fp8Buf& a, const Fp8Buf& b, const float* bias, const Tensor& c) {
+  return gemm_args(a.codes, a.scales(), b.codes, b.scales(), a.rows, b.rows, a.K, bias, c);
+}
+void fp8_product(Fp8GemmArgs g, const Tensor& c) {
+  g.ksplit = fp8_gemm_ksplit(g.M, g.N, g.K);
   Tensor slab;
   if (g.ksplit > 1) {
-    slab = torch::empty({(int64_t)g.ksplit, M, N}, c.options().dtype(torch::kFloat32));
+    slab = torch::empty({(int64_t)g.ksplit, g.M, g.N}, c.options().dtype(torch::kFloat32));
     g.slab = slab.data_ptr<float>();
   }
   launch_fp8_gemm(g, stream_of(c));
   launched();
-}
-void fp8_product(const Fp8Buf& a, const Fp8Buf& b, const float* bias, const Tensor& c) {
-  fp8_product(a.codes(), a.scales(), b.codes(), b.scales(), a.rows, b.rows, a.K, bias, c);
 }
 
 const float* bias_of(const Tensor& b, int64_t N, const Tensor& like) {
@@ -422,7 +437,7 @@ Tensor block_fp8_matmul(const Tensor& a, const Tensor& sa, const Tensor& b, cons
   c10::DeviceGuard guard(a.device());
   const Tensor bc = bias.has_value() ? bias->detach().contiguous() : Tensor();
   auto c = torch::empty({a.size(0), b.size(0)}, a.options().dtype(out));
-  fp8_product(bytes(a), bytes(sa), bytes(b), bytes(sb), a.size(0), b.size(0), K, bias_of(bc, b.size(0), a), c);
+  fp8_product(gemm_args(bytes(a), bytes(sa), bytes(b), bytes(sb), a.size(0), b.size(0), K, bias_of(bc, b.size(0), a), c), c);
   return c;
 }
 
@@ -436,13 +451,16 @@ Tensor block_fp8_fc_packed(const Tensor& x, const Tensor& codes, const Tensor& s
   fp8_dims(M, O);
   const Tensor xr = rows_of(x.detach(), M, K), bc = b.has_value() ? b->detach().contiguous() : Tensor();
   auto q = quant_args(xr, M, K, false);
-  const Fp8Buf xq = fp8_new(M, K, x);
-  q.row_codes = xq.codes();
+  Parts tmp;
+  tmp.add(Fp8Buf::bytes(M, K));
+  tmp.allocate(x);
+  const Fp8Buf xq = tmp.blocks(0, M, K);
+  q.row_codes = xq.codes;
   q.row_scales = xq.scales();
   launch_fp8_quant(q, stream_of(x));
   launched();
   auto y = torch::empty({M, O}, x.options().memory_format(c10::MemoryFormat::Contiguous));
-  fp8_product(xq.codes(), xq.scales(), bytes(codes), bytes(scales), M, O, K, bias_of(bc, O, x), y);
+  fp8_product(gemm_args(xq.codes, xq.scales(), bytes(codes), bytes(scales), M, O, K, bias_of(bc, O, x), y), y);
   return y;
 }
 
@@ -458,30 +476,36 @@ class Fp8FcFn : public torch::autograd::Function<Fp8FcFn> {
     const Tensor xr = rows_of(x, M, K), Wr = rows_of(W, K, O), bc = b.has_value() ? b->contiguous() : Tensor();
     const bool need_dx = grad && x.requires_grad(), need_dw = grad && W.requires_grad();
     auto s = stream_of(x);
-    const Fp8Buf wt = fp8_new(O, K, x), xq = fp8_new(M, K, x);
-    Fp8Buf wq, xt;
+    // the forward's own: codes of W^T and x; the backward's: codes of W (for dx) and x^T (for dW)
+    Parts tmp, kept;
+    const int64_t at_wt = tmp.add(Fp8Buf::bytes(O, K)), at_xq = tmp.add(Fp8Buf::bytes(M, K));
+    tmp.allocate(x);
+    const Fp8Buf wt = tmp.blocks(at_wt, O, K), xq = tmp.blocks(at_xq, M, K);
+    const int64_t at_wq = need_dx ? kept.add(Fp8Buf::bytes(K, O)) : 0, at_xt = need_dw ? kept.add(Fp8Buf::bytes(K, M)) : 0;
+    if (need_dx || need_dw) kept.allocate(x);
     auto qw = quant_args(Wr, K, O, true);
-    qw.col_codes = wt.codes();
+    qw.col_codes = wt.codes;
     qw.col_scales = wt.scales();
     if (need_dx) {
-      wq = fp8_new(K, O, x);
-      qw.row_codes = wq.codes();
+      const Fp8Buf wq = kept.blocks(at_wq, K, O);
+      qw.row_codes = wq.codes;
       qw.row_scales = wq.scales();
     }
-    launch_fp8_quant(qw, s);
     auto qx = quant_args(xr, M, K, false);
-    qx.row_codes = xq.codes();
+    qx.row_codes = xq.codes;
     qx.row_scales = xq.scales();
     if (need_dw) {
-      xt = fp8_new(K, M, x);
-      qx.col_codes = xt.codes();
+      const Fp8Buf xt = kept.blocks(at_xt, K, M);
+      qx.col_codes = xt.codes;
       qx.col_scales = xt.scales();
     }
-    launch_fp8_quant(qx, s);
+    launch_fp8_quant_two(qx, qw, s);
     launched();
     auto y = torch::empty({M, O}, x.options().memory_format(c10::MemoryFormat::Contiguous));
-    fp8_product(xq, wt, bias_of(bc, O, x), y);
-    ctx->save_for_backward({wq.mem, xt.mem});
+    fp8_product(gemm_args(xq, wt, bias_of(bc, O, x), y), y);
+    ctx->save_for_backward({kept.mem});
+    ctx->saved_data["wq"] = at_wq;
+    ctx->saved_data["xt"] = at_xt;
     ctx->saved_data["M"] = M;
     ctx->saved_data["K"] = K;
     ctx->saved_data["O"] = O;
@@ -499,38 +523,60 @@ class Fp8FcFn : public torch::autograd::Function<Fp8FcFn> {
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1),
                want_b = has_b && ctx->needs_input_grad(2);
     const Tensor dy = rows_of(g[0], M, O);
-    Tensor dx, dW, db, slab;
-    auto f32 = dy.options().dtype(torch::kFloat32);
+    Tensor dx, dW, db;
     auto q = quant_args(dy, M, O, false);
-    Fp8Buf dq, dt;
+    Parts tmp;
+    const int64_t at_dq = want_x ? tmp.add(Fp8Buf::bytes(M, O)) : 0, at_dt = want_w ? tmp.add(Fp8Buf::bytes(O, M)) : 0,
+                  at_slab = want_b ? tmp.add((M + 127) / 128 * O * 4) : 0;
+    if (want_x) dx = torch::empty({M, K}, dy.options());
+    if (want_w) dW = torch::empty({K, O}, dy.options().dtype((at::ScalarType)sd["wt"].toInt()));
+    if (want_b) db = torch::empty(sd["bs"].toIntVector(), dy.options().dtype(torch::kFloat32));
+    if (M == 0) {  // no row: the sums over rows are zero
+      if (want_w) dW.zero_();
+      if (want_b) db.zero_();
+      return {dx, dW, db, Tensor()};
+    }
+    if (!(want_x || want_w || want_b)) return {dx, dW, db, Tensor()};
+    uint8_t* kept = sv[0].defined() ? sv[0].data_ptr<uint8_t>() : nullptr;
+    // the products' arguments but for the temporaries' addresses, which the slices decide on
+    Fp8GemmArgs gx, gw;
+    bool two = false;
+    int64_t at_gx = 0, at_gw = 0;
+    const Fp8Buf wq{kept + sd["wq"].toInt(), K, O}, xt{kept + sd["xt"].toInt(), K, M};
+    if (want_x) gx = gemm_args(Fp8Buf{nullptr, M, O}, wq, nullptr, dx);
+    if (want_w) gw = gemm_args(xt, Fp8Buf{nullptr, O, M}, nullptr, dW);
+    if (want_x && want_w && fp8_gemm_two_split(gx, gw)) {
+      two = true;
+      if (gx.ksplit > 1) at_gx = tmp.add((int64_t)gx.ksplit * M * K * 4);
+      if (gw.ksplit > 1) at_gw = tmp.add((int64_t)gw.ksplit * K * O * 4);
+    }
+    tmp.allocate(dy);
+    const Fp8Buf dq = tmp.blocks(at_dq, M, O), dt = tmp.blocks(at_dt, O, M);
     if (want_x) {
-      dq = fp8_new(M, O, dy);
-      q.row_codes = dq.codes();
+      gx.a = q.row_codes = dq.codes;
       q.row_scales = dq.scales();
+      gx.sa = dq.scales();
     }
     if (want_w) {
-      dt = fp8_new(O, M, dy);
-      q.col_codes = dt.codes();
+      q.col_codes = dt.codes;
       q.col_scales = dt.scales();
+      gw.b = dt.codes;
+      gw.sb = dt.scales();
     }
     if (want_b) {
-      db = M ? torch::empty(sd["bs"].toIntVector(), f32) : torch::zeros(sd["bs"].toIntVector(), f32);
-      slab = torch::empty({(M + 127) / 128, O}, f32);
-      q.colsum = db.data_ptr<float>();
-      q.slab = slab.data_ptr<float>();
+      q.slab = reinterpret_cast<float*>(tmp.at(at_slab));
+      if (!two) q.colsum = db.data_ptr<float>();
     }
-    if (want_x || want_w || want_b) {
-      launch_fp8_quant(q, stream_of(dy));
+    launch_fp8_quant(q, stream_of(dy));
+    launched();
+    if (two) {
+      gx.slab = reinterpret_cast<float*>(tmp.at(at_gx));
+      gw.slab = reinterpret_cast<float*>(tmp.at(at_gw));
+      launch_fp8_gemm_two(gx, gw, q.slab, (M + 127) / 128, O, want_b ? db.data_ptr<float>() : nullptr, stream_of(dy));
       launched();
-    }
-    if (want_x) {
-      dx = torch::empty({M, K}, dy.options());
-      fp8_product(dq, fp8_buf(sv[0], K, O), nullptr, dx);
-    }
-    if (want_w) {
-      dW = torch::empty({K, O}, dy.options().dtype((at::ScalarType)sd["wt"].toInt()));
-      if (M) fp8_product(fp8_buf(sv[1], K, M), dt, nullptr, dW);
-      else dW.zero_();
+    } else {
+      if (want_x) fp8_product(gx, dx);
+      if (want_w) fp8_product(gw, dW);
     }
     return {dx, dW, db, Tensor()};
   }

@@ -200,12 +200,13 @@ __device__ __forceinline__ uint32_t max16(uint32_t m) {
 // transposed codes, put together through LDS so that whole 128-byte lines are
 // written.
 template <typename E>
-__global__ __launch_bounds__(256, sizeof(E) == 4 ? 3 : 4) void k_fp8_quant_tile(Fp8QuantArgs a) {
+__device__ __forceinline__ void quant_tile(const Fp8QuantArgs& a, int tile) {
   using X = Eight<E>;
   __shared__ __attribute__((aligned(16))) uint8_t cols[128 * 128];
   __shared__ __attribute__((aligned(16))) uint32_t red[4][X::NM * 16];
   __shared__ uint32_t wave_max[4];
-  const int64_t k0 = (int64_t)blockIdx.x * 128, m0 = (int64_t)blockIdx.y * 128;
+  const int kbs = (int)(fp8_kp(a.K) / 128), mbs = (int)(fp8_kp(a.M) / 128), bx = tile % kbs, by = tile / kbs;
+  const int64_t k0 = (int64_t)bx * 128, m0 = (int64_t)by * 128;
   const int t = threadIdx.x, cl = t & 15, g = t >> 4, c0 = cl * 8, wave = t >> 6;
   const int64_t rows = a.M - m0, width = a.K - k0;
   const int64_t kp = fp8_kp(a.K), ksp = fp8_sp(a.K), mp = fp8_kp(a.M), msp = fp8_sp(a.M);
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 3 : 4) void k_fp8_quant_tile(
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) s += part[i * 128 + t];
-      a.slab[(int64_t)blockIdx.y * a.K + k0 + t] = s;
+      a.slab[(int64_t)by * a.K + k0 + t] = s;
     }
     __syncthreads();
   }
@@ -288,9 +289,9 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 3 : 4) void k_fp8_quant_tile(
       *reinterpret_cast<uint2*>(a.row_codes + (m0 + r) * kp + k0 + c0) = x[i].row_codes(scale);
       if (cl == 0) {
         uint8_t* s = a.row_scales + (m0 + r) * ksp;
-        s[blockIdx.x] = (uint8_t)byte;
-        if (blockIdx.x == gridDim.x - 1)
-          for (int64_t q = gridDim.x; q < ksp; ++q) s[q] = 127;
+        s[bx] = (uint8_t)byte;
+        if (bx == kbs - 1)
+          for (int64_t q = kbs; q < ksp; ++q) s[q] = 127;
       }
     }
   }
@@ -323,9 +324,9 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 3 : 4) void k_fp8_quant_tile(
           make_uint2(X::col_codes(x, j, scale), X::col_codes(x + 4, j, scale));
       if (g == 0 && c < width) {
         uint8_t* s = a.col_scales + (k0 + c) * msp;
-        s[blockIdx.y] = (uint8_t)byte;
-        if (blockIdx.y == gridDim.y - 1)
-          for (int64_t q = gridDim.y; q < msp; ++q) s[q] = 127;
+        s[by] = (uint8_t)byte;
+        if (by == mbs - 1)
+          for (int64_t q = mbs; q < msp; ++q) s[q] = 127;
       }
     }
     __syncthreads();
@@ -337,6 +338,17 @@ __global__ __launch_bounds__(256, sizeof(E) == 4 ? 3 : 4) void k_fp8_quant_tile(
             *reinterpret_cast<const uint4*>(cols + c * 128 + ((w ^ c >> 3) & 7) * 16);
     }
   }
+}
+
+template <typename E>
+__global__ __launch_bounds__(256, sizeof(E) == 4 ? 3 : 4) void k_fp8_quant_tile(Fp8QuantArgs a) {
+  quant_tile<E>(a, blockIdx.x);
+}
+// two matrices in one launch (the activations and the weight of a forward): the second one's tiles come behind
+template <typename E, typename W>
+__global__ __launch_bounds__(256, 3) void k_fp8_quant_two(Fp8QuantArgs a, Fp8QuantArgs w, int tiles) {
+  if ((int)blockIdx.x < tiles) quant_tile<E>(a, blockIdx.x);
+  else quant_tile<W>(w, blockIdx.x - tiles);
 }
 
 // ---------------------------------------------------------------- product
@@ -463,24 +475,31 @@ __device__ __forceinline__ void block_barrier() {
 // writes lanes in order, so the turn is made in the global address.  The
 // exponent bytes come by DMA too, the dwords of four blocks at once and four
 // blocks ahead.
+template <int WR, int WC, int MT, int NT>
+struct Fp8Tile {
+  static constexpr int kThreads = 64 * WR * WC, kRows = (WR * MT + WC * NT) * 32;
+  __attribute__((aligned(16))) uint8_t lds[2 * kRows * 128];
+  uint32_t words[2][kRows];
+};
+// workgroup `wg` of the g.ksplit slices of all tiles
 template <int WR, int WC, int MT, int NT, typename C>
-__global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
+__device__ __forceinline__ void gemm_tile(const Fp8GemmArgs& g, Fp8Tile<WR, WC, MT, NT>& shared, int wg) {
   constexpr bool FULL = std::is_same<C, float>::value;
   using F = Frag<FULL>;
   constexpr int BM = WR * MT * 32, BN = WC * NT * 32, W = WR * WC, ROWS = BM + BN, BLOCK = ROWS * 128;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BLOCK];
-  __shared__ uint32_t words[2][ROWS];
+  auto& lds = shared.lds;
+  auto& words = shared.words;
   const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wr = w / WC, wc = w % WC;
   // the 8 XCDs take workgroups in turn: give each a run of tiles, 8 rows of tiles deep, that share operands in its L2
   const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN, tiles = tm * tn;
-  const int q = tiles / 8, rr = tiles % 8, xcd = blockIdx.x % 8;
-  const int id = (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + blockIdx.x / 8;
+  const int slice = wg / tiles, at = wg % tiles, q = tiles / 8, rr = tiles % 8, xcd = at % 8;
+  const int id = (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + at / 8;
   const int band = id / (8 * tn), deep = min(8, tm - band * 8), in = id - band * 8 * tn;
   const int m0 = (band * 8 + in % deep) * BM, n0 = in / deep * BN;
   const int64_t kp = fp8_kp(g.K), sp = fp8_sp(g.K);
   const int nb = (int)(kp / 128), per = fp8_slice(nb, g.ksplit);
-  const int kb0 = blockIdx.z * per, kb1 = min(nb, kb0 + per);  // kb0 is a multiple of 4; no slice is empty
+  const int kb0 = slice * per, kb1 = min(nb, kb0 + per);  // kb0 is a multiple of 4; no slice is empty
   constexpr int LA = BM / 8 / W, LB = BN / 8 / W;              // DMAs of 8 rows a wave and block
   static_assert(BM % (8 * W) == 0 && BN % (8 * W) == 0, "whole loads");
   constexpr int LS = ROWS / 64 / W;  // DMAs of 64 dwords a wave and four blocks
@@ -621,7 +640,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
     constexpr int TILES = PART / (PIECES * 16) / 32 < MT ? PART / (PIECES * 16) / 32 : MT;  // instruction tiles at a time
     static_assert(TILES >= 1 && MT % TILES == 0 && 64 % PIECES == 0, "whole passes");
     uint8_t* mine = lds + w * PART;
-    O* c = g.ksplit > 1 ? (O*)(g.slab + (int64_t)blockIdx.z * g.M * g.N) : (O*)g.c;
+    O* c = g.ksplit > 1 ? (O*)(g.slab + (int64_t)slice * g.M * g.N) : (O*)g.c;
     const int nw = n0 + wc * NT * 32;
 #pragma unroll
     for (int i0 = 0; i0 < MT; i0 += TILES) {
@@ -661,10 +680,23 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
   else leave(C(0), g.bias != nullptr);
 }
 
-// c = sum of the slices in order (+ bias)
+template <int WR, int WC, int MT, int NT, typename C>
+__global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8GemmArgs g) {
+  __shared__ Fp8Tile<WR, WC, MT, NT> shared;
+  gemm_tile<WR, WC, MT, NT, C>(g, shared, blockIdx.x);
+}
+// two products in one launch (a backward's dx and dW): neither fills the card alone
+template <typename C, typename D>
+__global__ __launch_bounds__(256) void k_fp8_gemm_two(Fp8GemmArgs g, Fp8GemmArgs h, int wgs) {
+  __shared__ Fp8Tile<2, 2, 2, 2> shared;
+  if ((int)blockIdx.x < wgs) gemm_tile<2, 2, 2, 2, C>(g, shared, blockIdx.x);
+  else gemm_tile<2, 2, 2, 2, D>(h, shared, blockIdx.x - wgs);
+}
+
+// c = sum of the slices in order (+ bias), 4 columns a thread
 template <typename C>
-__global__ __launch_bounds__(256) void k_fp8_join(Fp8GemmArgs g) {
-  const int64_t n4 = ((int64_t)g.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__device__ __forceinline__ void join_slices(const Fp8GemmArgs& g, int64_t i) {
+  const int64_t n4 = ((int64_t)g.N + 3) / 4;
   if (i >= n4 * g.M) return;
   const int64_t m = i / n4;
   const int n = (int)(i % n4) * 4;
@@ -681,6 +713,37 @@ __global__ __launch_bounds__(256) void k_fp8_join(Fp8GemmArgs g) {
     }
   }
   store4((C*)g.c + m * g.N + n, g.N - n, s + bias4(g.bias, n, g.N));
+}
+inline __host__ __device__ int64_t join_wgs(const Fp8GemmArgs& g) {
+  return g.ksplit > 1 ? (((int64_t)g.N + 3) / 4 * g.M + 255) / 256 : 0;
+}
+template <typename C>
+__global__ __launch_bounds__(256) void k_fp8_join(Fp8GemmArgs g) {
+  join_slices<C>(g, (int64_t)blockIdx.x * 256 + threadIdx.x);
+}
+// what is left of a backward behind its products, in one launch: the slices of dx and of dW, and db = column sums of
+// the quantiser's slab [rows][K], in an order of the rows' number alone (64 columns a workgroup, 4 waves)
+template <typename C, typename D>
+__global__ __launch_bounds__(256) void k_fp8_finish(Fp8GemmArgs g, Fp8GemmArgs h, const float* slab, int rows, int K,
+                                                    float* db) {
+  int64_t wg = blockIdx.x;
+  if (wg < join_wgs(g)) return join_slices<C>(g, wg * 256 + threadIdx.x);
+  wg -= join_wgs(g);
+  if (wg < join_wgs(h)) return join_slices<D>(h, wg * 256 + threadIdx.x);
+  wg -= join_wgs(h);
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = (int)wg * 64 + lane;
+  float s[8] = {};
+  if (c < K) {
+    int r = w;
+    for (; r + 28 < rows; r += 32)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += slab[(int64_t)(r + 4 * i) * K + c];
+    for (; r < rows; r += 4) s[0] += slab[(int64_t)r * K + c];
+  }
+  red[w][lane] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+  __syncthreads();
+  if (w == 0 && c < K) db[c] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
 
 // Up to 16 MT rows of a: the bytes of b are the cost, so they go straight to
@@ -769,65 +832,119 @@ void skinny(const Fp8GemmArgs& g, hipStream_t s) {
   else hipLaunchKernelGGL((k_fp8_skinny<4, NT, C>), grid, dim3(512), 0, s, g);
 }
 
-template <typename C>
-void gemm(const Fp8GemmArgs& g, hipStream_t s) {
-  if (g.M <= 64) {
-    if (g.M > 16 && g.N >= 4096) skinny<2, C>(g, s);
-    else skinny<1, C>(g, s);
-    return;
-  }
-  auto tiles = [&](int bm, int bn) { return dim3((unsigned)((int64_t)((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn)), 1, g.ksplit); };
-  if ((int64_t)g.M * g.N >= (int64_t)256 * 256 * 192) {
-    hipLaunchKernelGGL((k_fp8_gemm<2, 2, 4, 4, C>), tiles(256, 256), dim3(256), 0, s, g);
-  } else {
-    hipLaunchKernelGGL((k_fp8_gemm<2, 2, 2, 2, C>), tiles(128, 128), dim3(256), 0, s, g);
-  }
-  if (g.ksplit > 1) {
-    const int64_t n = ((int64_t)g.N + 3) / 4 * g.M;
-    hipLaunchKernelGGL(k_fp8_join<C>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, g);
-  }
-}
+// Few rows of a: a launch that only streams b.  With few rows of b as well and a long K (a narrow weight's gradient)
+// its workgroups are too few: tiles in slices of K then.
+bool is_skinny(int M, int N, int64_t K) { return M <= 64 && (N >= 2048 || K <= 16384); }
+// 256 x 256 tiles from the sizes where they fill the card: 8192^3 to bf16 takes 481 us in them, 640 in 128 x 128
+bool is_large(const Fp8GemmArgs& g) { return (int64_t)g.M * g.N >= (int64_t)256 * 256 * 192; }
+int64_t small_tiles(const Fp8GemmArgs& g) { return (int64_t)((g.M + 127) / 128) * ((g.N + 127) / 128); }
 
-}  // namespace
-
-int fp8_gemm_ksplit(int M, int N, int64_t K) {
-  if (M <= 64) return 1;
-  const int64_t tiles = (int64_t)((M + 127) / 128) * ((N + 127) / 128), nb = fp8_kp(K) / 128;
-  // about one workgroup a CU, at least 4 blocks of K each
-  int64_t split = 256 / tiles;
+// slices of K so that the tiles come to about `want` workgroups, at least 4 blocks each
+int slices(int64_t tiles, int64_t K, int64_t want) {
+  const int64_t nb = fp8_kp(K) / 128;
+  int64_t split = want / tiles;
   if (split > nb / 4) split = nb / 4;
   if (split < 1) split = 1;
   const int per = fp8_slice((int)nb, (int)split);
   return (int)((nb + per - 1) / per);  // no empty slice
 }
 
-void launch_fp8_gemm(const Fp8GemmArgs& g, hipStream_t s) {
-  if (g.M == 0 || g.N == 0) return;
-  if (g.ct == kF32) gemm<float>(g, s);
-  else if (g.ct == kBF16) gemm<__bf16>(g, s);
-  else gemm<_Float16>(g, s);
+template <typename C>
+void gemm(const Fp8GemmArgs& g, hipStream_t s) {
+  if (is_skinny(g.M, g.N, g.K)) {
+    if (g.M > 16 && g.N >= 4096) skinny<2, C>(g, s);
+    else skinny<1, C>(g, s);
+    return;
+  }
+  if (is_large(g)) {
+    const dim3 grid((unsigned)((int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256) * g.ksplit));
+    hipLaunchKernelGGL((k_fp8_gemm<2, 2, 4, 4, C>), grid, dim3(256), 0, s, g);
+  } else {
+    hipLaunchKernelGGL((k_fp8_gemm<2, 2, 2, 2, C>), dim3((unsigned)(small_tiles(g) * g.ksplit)), dim3(256), 0, s, g);
+  }
+  if (g.ksplit > 1) hipLaunchKernelGGL(k_fp8_join<C>, dim3((unsigned)join_wgs(g)), dim3(256), 0, s, g);
 }
 
-namespace {
+template <typename F>
+void by_type(BlockType t, F f) {
+  if (t == kF32) f(float{});
+  else if (t == kBF16) f(__bf16{});
+  else f(_Float16{});
+}
+// a type and the same or fp32: what a weight may be beside its activations
+template <typename F>
+bool by_types(BlockType t, BlockType w, F f) {
+  if (w != t && w != kF32) return false;
+  by_type(t, [&](auto e) {
+    if (w == kF32) f(e, float{});
+    else f(e, e);
+  });
+  return true;
+}
+
 template <typename E>
 void quant(const Fp8QuantArgs& a, hipStream_t s) {
-  const int64_t kb = fp8_kp(a.K) / 128;
-  if (!a.col_codes && !a.colsum && !a.tile) {
+  const int64_t kb = fp8_kp(a.K) / 128, mb = fp8_kp(a.M) / 128;
+  if (!a.col_codes && !a.slab && !a.tile) {
     hipLaunchKernelGGL(k_fp8_quant_rows<E>, dim3((unsigned)((a.M * kb + 15) / 16)), dim3(256), 0, s, a);
     return;
   }
-  const int64_t mb = (a.M + 127) / 128;
-  hipLaunchKernelGGL(k_fp8_quant_tile<E>, dim3((unsigned)kb, (unsigned)mb), dim3(256), 0, s, a);
-  if (a.colsum)
-    launch_block_cols(a.slab, mb, a.K, &a.colsum, 1, a.K, s);
+  hipLaunchKernelGGL(k_fp8_quant_tile<E>, dim3((unsigned)(kb * mb)), dim3(256), 0, s, a);
+  if (a.colsum) launch_block_cols(a.slab, mb, a.K, &a.colsum, 1, a.K, s);
 }
+
 }  // namespace
+
+int fp8_gemm_ksplit(int M, int N, int64_t K) {
+  Fp8GemmArgs g;
+  g.M = M;
+  g.N = N;
+  if (is_skinny(M, N, K) || is_large(g)) return 1;
+  return slices(small_tiles(g), K, 256);
+}
+
+bool fp8_gemm_two_split(Fp8GemmArgs& g, Fp8GemmArgs& h) {
+  if (is_large(g) || is_large(h) || g.M <= 64 || (h.ct != g.ct && h.ct != kF32)) return false;
+  // two workgroups of 66 KB of LDS fit a CU; h (the long sum of dW) takes what g leaves of them
+  g.ksplit = slices(small_tiles(g), g.K, 256);
+  const int64_t left = 512 - small_tiles(g) * g.ksplit;
+  h.ksplit = slices(small_tiles(h), h.K, left > 256 ? left : 256);
+  return true;
+}
+
+void launch_fp8_gemm_two(const Fp8GemmArgs& g, const Fp8GemmArgs& h, const float* slab, int64_t rows, int64_t K, float* db,
+                         hipStream_t s) {
+  by_types(g.ct, h.ct, [&](auto c, auto d) {
+    using C = decltype(c);
+    using D = decltype(d);
+    const int64_t n = small_tiles(g) * g.ksplit;
+    hipLaunchKernelGGL((k_fp8_gemm_two<C, D>), dim3((unsigned)(n + small_tiles(h) * h.ksplit)), dim3(256), 0, s, g, h, (int)n);
+    const int64_t left = join_wgs(g) + join_wgs(h) + (db ? (K + 63) / 64 : 0);
+    if (left)
+      hipLaunchKernelGGL((k_fp8_finish<C, D>), dim3((unsigned)left), dim3(256), 0, s, g, h, slab, (int)rows, (int)K, db);
+  });
+}
+
+void launch_fp8_gemm(const Fp8GemmArgs& g, hipStream_t s) {
+  if (g.M == 0 || g.N == 0) return;
+  by_type(g.ct, [&](auto c) { gemm<decltype(c)>(g, s); });
+}
 
 void launch_fp8_quant(const Fp8QuantArgs& a, hipStream_t s) {
   if (a.M == 0 || a.K == 0) return;
-  if (a.t == kF32) quant<float>(a, s);
-  else if (a.t == kBF16) quant<__bf16>(a, s);
-  else quant<_Float16>(a, s);
+  by_type(a.t, [&](auto e) { quant<decltype(e)>(a, s); });
+}
+
+void launch_fp8_quant_two(const Fp8QuantArgs& a, const Fp8QuantArgs& w, hipStream_t s) {
+  const bool tiles = a.M && w.M && (a.col_codes || a.tile) && !a.slab && !w.slab;
+  const int64_t n = fp8_kp(a.K) / 128 * (fp8_kp(a.M) / 128), m = fp8_kp(w.K) / 128 * (fp8_kp(w.M) / 128);
+  // many tiles fill the card by themselves, and a 16-bit type has more of them on a CU in its own kernel
+  if (tiles && n <= 1024 && by_types(a.t, w.t, [&](auto e, auto f) {
+        hipLaunchKernelGGL((k_fp8_quant_two<decltype(e), decltype(f)>), dim3((unsigned)(n + m)), dim3(256), 0, s, a, w, (int)n);
+      }))
+    return;
+  launch_fp8_quant(w, s);
+  launch_fp8_quant(a, s);
 }
 
 }  // namespace pbx

@@ -96,10 +96,12 @@ struct Fp8QuantArgs {
   int tile = 0;  // one scale for 128 x 128, both outputs alike
   uint8_t *row_codes = nullptr, *row_scales = nullptr;  // x in blocks along K: [M][fp8_kp(K)], [M][fp8_sp(K)]
   uint8_t *col_codes = nullptr, *col_scales = nullptr;  // x^T in blocks along M: [K][fp8_kp(M)], [K][fp8_sp(M)]
-  float* colsum = nullptr;                              // [K] fp32 column sums of x
-  float* slab = nullptr;                                // [ceil(M / 128)][K] for them
+  float* slab = nullptr;    // [ceil(M / 128)][K]: column sums of x by tiles of rows
+  float* colsum = nullptr;  // [K] fp32: their sums (null: the caller adds the slab up)
 };
 void launch_fp8_quant(const Fp8QuantArgs& a, hipStream_t s);
+// activations and weight (in 128 x 128 blocks) of one layer, in one launch where their kernel is the same
+void launch_fp8_quant_two(const Fp8QuantArgs& a, const Fp8QuantArgs& w, hipStream_t s);
 
 struct Fp8GemmArgs {  // c [M, N] = a [M, K] b [N, K]^T (+ bias [N])
   const uint8_t *a = nullptr, *b = nullptr, *sa = nullptr, *sb = nullptr;
@@ -115,6 +117,11 @@ struct Fp8GemmArgs {  // c [M, N] = a [M, K] b [N, K]^T (+ bias [N])
 PBX_FP8_HD int fp8_slice(int blocks, int ksplit) { return ((blocks + ksplit - 1) / ksplit + 3) / 4 * 4; }
 int fp8_gemm_ksplit(int M, int N, int64_t K);
 void launch_fp8_gemm(const Fp8GemmArgs& a, hipStream_t s);
+// Two products of one layer's backward (dx, dW) in one launch, and a second one that joins their slices and sums db
+// [K] from the quantiser's slab.  _split says whether they go together, and into how many slices each.
+bool fp8_gemm_two_split(Fp8GemmArgs& g, Fp8GemmArgs& h);
+void launch_fp8_gemm_two(const Fp8GemmArgs& g, const Fp8GemmArgs& h, const float* slab, int64_t rows, int64_t K, float* db,
+                         hipStream_t s);
 
 #ifdef __HIPCC__
 // ---------------------------------------------------------------- device helpers
