@@ -424,10 +424,14 @@ __device__ __forceinline__ void store4(C* p, int valid, f32x4 v) {
   }
 }
 __device__ __forceinline__ f32x4 bias4(const float* b, int n, int N) {
+  typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
   f32x4 v{0.f, 0.f, 0.f, 0.f};
-  if (b) {
+  if (b && n + 4 <= N) {
+    v = *reinterpret_cast<const vec*>(b + n);
+  } else if (b) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = n + j < N ? b[n + j] : 0.f;
+    for (int j = 0; j < 4; ++j)
+      if (n + j < N) v[j] = b[n + j];
   }
   return v;
 }
@@ -539,13 +543,20 @@ __device__ __forceinline__ void gemm_tile(const Fp8GemmArgs& g, Fp8Tile<WR, WC, 
 #pragma unroll
     for (int j = 0; j < NT; ++j) sb[j] = words[kb >> 2 & 1][BM + (wc * NT + j) * 32 + fr];
   };
-  f32x16 acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
+  f32x16 acc[MT][NT];  // the sums begin with the bias: it costs nothing behind the first DMAs, and 3 us a tile at the end
+  const float* bias = g.ksplit == 1 ? g.bias : nullptr;
+  auto begin = [&]() {
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 v = bias4(bias, n0 + (wc * NT + j) * 32 + r * 8 + fh * 4, g.N);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][4 * r + e] = v[e];
+      }
+  };
   i32x8 fa[2][MT], fb[2][NT];  // of the two halves
   const uint8_t *fbase = lds + (wr * MT * 32 + fr) * 128, *gbase = lds + (BM + wc * NT * 32 + fr) * 128;
   int pos[2][2];
@@ -616,6 +627,7 @@ __device__ __forceinline__ void gemm_tile(const Fp8GemmArgs& g, Fp8Tile<WR, WC, 
   fill_words(kb0);
   fill(0, kb0);
   fill(1, kb0 + 1);
+  begin();
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
   block_barrier();
   read_words(kb0);
@@ -632,7 +644,7 @@ __device__ __forceinline__ void gemm_tile(const Fp8GemmArgs& g, Fp8Tile<WR, WC, 
   block_barrier();
   // A wave turns its tile through its own part of LDS, so that rows leave in whole lines: 16-byte piece p of row r at
   // place p ^ r (as far as there are pieces), which spreads both ways over the banks.
-  auto leave = [&](auto out, bool bias) {
+  auto leave = [&](auto out) {
     typedef decltype(out) O;
     typedef O vec __attribute__((ext_vector_type(16 / sizeof(O)), aligned(sizeof(O))));
     typedef O vec4 __attribute__((ext_vector_type(4)));
@@ -645,20 +657,20 @@ __device__ __forceinline__ void gemm_tile(const Fp8GemmArgs& g, Fp8Tile<WR, WC, 
 #pragma unroll
     for (int i0 = 0; i0 < MT; i0 += TILES) {
 #pragma unroll
-      for (int i = 0; i < TILES; ++i)
+      for (int j = 0; j < NT; ++j) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int i = 0; i < TILES; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int row = i * 32 + fr, col = j * 32 + r * 8 + fh * 4;
-            f32x4 v{acc[i0 + i][j][4 * r], acc[i0 + i][j][4 * r + 1], acc[i0 + i][j][4 * r + 2], acc[i0 + i][j][4 * r + 3]};
-            if (bias) v += bias4(g.bias, nw + col, g.N);
+            const f32x4 v{acc[i0 + i][j][4 * r], acc[i0 + i][j][4 * r + 1], acc[i0 + i][j][4 * r + 2], acc[i0 + i][j][4 * r + 3]};
             vec4 x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = (O)v[e];
             *reinterpret_cast<vec4*>(mine + row * PIECES * 16 + ((col / PER) ^ (row & (PIECES - 1))) * 16 +
                                      col % PER * sizeof(O)) = x;
           }
+      }
       const int mw = m0 + (wr * MT + i0) * 32;
 #pragma unroll 4
       for (int q = 0; q < TILES * 32 * PIECES / 64; ++q) {
@@ -676,8 +688,8 @@ __device__ __forceinline__ void gemm_tile(const Fp8GemmArgs& g, Fp8Tile<WR, WC, 
       }
     }
   };
-  if (g.ksplit > 1) leave(float(0), false);
-  else leave(C(0), g.bias != nullptr);
+  if (g.ksplit > 1) leave(float(0));
+  else leave(C(0));
 }
 
 template <int WR, int WC, int MT, int NT, typename C>
