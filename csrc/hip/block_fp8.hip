@@ -758,26 +758,19 @@ __global__ __launch_bounds__(256) void k_fp8_finish(Fp8GemmArgs g, Fp8GemmArgs h
   if (w == 0 && c < K) db[c] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
 
-// Up to 16 MT rows of a: the bytes of b are the cost, so they go straight to
-// registers, three blocks ahead.  A workgroup takes 16 NT rows of b; its 8
-// waves share the blocks of K and join their sums through LDS in order.  Two
-// tiles of b a wave halve the reads of a, which come from the L2 for every
-// workgroup.
+// Sums of 16 MT rows of a against 16 NT rows of b from n0 over the blocks [b0, b1) of K, by one wave: both go straight
+// to registers, three blocks ahead.
 template <int MT, int NT, typename C>
-__global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
+__device__ __forceinline__ void stream_blocks(const Fp8GemmArgs& g, int n0, int b0, int b1, f32x4 (&acc)[NT][MT]) {
   using F = Frag<std::is_same<C, float>::value>;
   constexpr int AHEAD = 3;
-  __shared__ f32x4 part[8][NT * MT][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 15, fg = lane >> 4;
+  const int lane = threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
   const int64_t kp = fp8_kp(g.K), sp = fp8_sp(g.K);
-  const int nb = (int)(kp / 128), b0 = (int)((int64_t)nb * w / 8), b1 = (int)((int64_t)nb * (w + 1) / 8);
-  const int n0 = blockIdx.x * 16 * NT;
   const uint8_t *pa[MT], *psa[MT], *pb[NT], *psb[NT];
-  f32x4 acc[NT][MT];
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     const int64_t r = min(n0 + j * 16 + fr, g.N - 1);
-    pb[j] = g.b + r * kp + fg * 32;
+    pb[j] = g.b + r * kp + fg * 16;
     psb[j] = g.sb + r * sp;
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -785,7 +778,7 @@ __global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int64_t r = min(i * 16 + fr, g.M - 1);
-    pa[i] = g.a + r * kp + fg * 32;
+    pa[i] = g.a + r * kp + fg * 16;
     psa[i] = g.sa + r * sp;
   }
   i32x8 va[AHEAD][MT], vb[AHEAD][NT];
@@ -793,12 +786,12 @@ __global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
   auto load = [&](int at, int kb) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      vb[at][j] = codes32(pb[j] + (int64_t)kb * 128, pb[j] + (int64_t)kb * 128 + 16);
+      vb[at][j] = codes32(pb[j] + (int64_t)kb * 128, pb[j] + (int64_t)kb * 128 + 64);
       eb[at][j] = psb[j][kb];
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      va[at][i] = codes32(pa[i] + (int64_t)kb * 128, pa[i] + (int64_t)kb * 128 + 16);
+      va[at][i] = codes32(pa[i] + (int64_t)kb * 128, pa[i] + (int64_t)kb * 128 + 64);
       ea[at][i] = psa[i][kb];
     }
   };
@@ -821,32 +814,45 @@ __global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
       if (kb + u + AHEAD < b1) load(u, kb + u + AHEAD);
     }
   }
+}
+
+// Up to 16 MT rows of a in one launch: the bytes of b are the cost.  A
+// workgroup takes 16 rows of b; its 8 waves share the blocks of K and join
+// their sums through LDS in order.
+template <int MT, typename C>
+__global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
+  __shared__ f32x4 part[8][MT][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nb = (int)(fp8_kp(g.K) / 128), n0 = blockIdx.x * 16;
+  f32x4 acc[1][MT];
+  stream_blocks<MT, 1, C>(g, n0, (int)((int64_t)nb * w / 8), (int)((int64_t)nb * (w + 1) / 8), acc);
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) part[w][j * MT + i][lane] = acc[j][i];
+  for (int i = 0; i < MT; ++i) part[w][i][lane] = acc[0][i];
   __syncthreads();
-  if (w < NT * MT) {
+  if (w < MT) {
     f32x4 s = part[0][w][lane];
 #pragma unroll
     for (int k = 1; k < 8; ++k) s += part[k][w][lane];
-    const int m = w % MT * 16 + fr, n = n0 + w / MT * 16 + fg * 4;
+    const int m = w * 16 + (lane & 15), n = n0 + (lane >> 4) * 4;
     if (m < g.M && n < g.N) store4((C*)g.c + (int64_t)m * g.N + n, g.N - n, s + bias4(g.bias, n, g.N));
   }
 }
 
-template <int NT, typename C>
-void skinny(const Fp8GemmArgs& g, hipStream_t s) {
-  const dim3 grid((g.N + 16 * NT - 1) / (16 * NT));
-  if (g.M <= 16) hipLaunchKernelGGL((k_fp8_skinny<1, NT, C>), grid, dim3(512), 0, s, g);
-  else if (g.M <= 32) hipLaunchKernelGGL((k_fp8_skinny<2, NT, C>), grid, dim3(512), 0, s, g);
-  else if (g.M <= 48) hipLaunchKernelGGL((k_fp8_skinny<3, NT, C>), grid, dim3(512), 0, s, g);
-  else hipLaunchKernelGGL((k_fp8_skinny<4, NT, C>), grid, dim3(512), 0, s, g);
+// the number of 16-row tiles as a constant
+template <typename F>
+void by_rows(int M, F f) {
+  if (M <= 16) f(std::integral_constant<int, 1>{});
+  else if (M <= 32) f(std::integral_constant<int, 2>{});
+  else if (M <= 48) f(std::integral_constant<int, 3>{});
+  else f(std::integral_constant<int, 4>{});
 }
 
-// Few rows of a: a launch that only streams b.  With few rows of b as well and a long K (a narrow weight's gradient)
-// its workgroups are too few: tiles in slices of K then.
-bool is_skinny(int M, int N, int64_t K) { return M <= 64 && (N >= 2048 || K <= 16384); }
+// Few rows of a go through k_fp8_skinny, one launch that streams b, unless b is large (every workgroup reads a: 48 x
+// 8192 x 8192 takes 34 us there and 27 in tiles with K in slices; 33 x 1024 x 1024 6 against 9) or so narrow that its
+// workgroups are too few for a long K (64 x 64 x 16384: 54 against 18).  Up to 16 rows both take the same time.
+bool is_skinny(int M, int N, int64_t K) {
+  if (M > 64 || (N < 1024 && K > 4096)) return false;
+  return M <= 16 || (int64_t)N * K <= (int64_t)16 << 20;
+}
 // 256 x 256 tiles from the sizes where they fill the card: 8192^3 to bf16 takes 481 us in them, 640 in 128 x 128
 bool is_large(const Fp8GemmArgs& g) { return (int64_t)g.M * g.N >= (int64_t)256 * 256 * 192; }
 int64_t small_tiles(const Fp8GemmArgs& g) { return (int64_t)((g.M + 127) / 128) * ((g.N + 127) / 128); }
@@ -864,8 +870,9 @@ int slices(int64_t tiles, int64_t K, int64_t want) {
 template <typename C>
 void gemm(const Fp8GemmArgs& g, hipStream_t s) {
   if (is_skinny(g.M, g.N, g.K)) {
-    if (g.M > 16 && g.N >= 4096) skinny<2, C>(g, s);
-    else skinny<1, C>(g, s);
+    by_rows(g.M, [&](auto mt) {
+      hipLaunchKernelGGL((k_fp8_skinny<decltype(mt)::value, C>), dim3((unsigned)((g.N + 15) / 16)), dim3(512), 0, s, g);
+    });
     return;
   }
   if (is_large(g)) {
