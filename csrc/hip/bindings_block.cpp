@@ -108,19 +108,33 @@ class DropoutFn : public torch::autograd::Function<DropoutFn> {
   }
 };
 
-// whether an autograd node will be recorded for these inputs
-bool wants_grad(std::initializer_list<OptTensor> ts) {
+// Whether an autograd node will be recorded for these inputs.  While the
+// stream captures, a leaf whose accumulator an eager graph on the default
+// stream keeps alive is refused: the backward would hand its gradient over to
+// that stream, which may not take part in a capture, and end the process.
+bool wants_grad(std::initializer_list<OptTensor> ts, const Tensor& like) {
   if (!at::GradMode::is_enabled()) return false;
-  for (const OptTensor& t : ts)
-    if (t.has_value() && t->requires_grad()) return true;
-  return false;
+  bool any = false;
+  for (const OptTensor& t : ts) any |= t.has_value() && t->requires_grad();
+  if (!any) return false;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  C10_HIP_CHECK(hipStreamIsCapturing(stream_of(like), &status));
+  if (status == hipStreamCaptureStatusNone) return true;
+  for (const OptTensor& t : ts) {
+    if (!t.has_value() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto s = acc ? acc->stream() : c10::nullopt;
+    BK_CHECK(!s.has_value() || s->id() != 0,
+             "the stream captures a graph while an eager autograd graph of the same leaf is alive; drop its outputs first");
+  }
+  return true;
 }
 
 Tensor block_dropout(const Tensor& x, const OptTensor& seed, int64_t thr, double up, int64_t seed_v,
                      int64_t offset_v) {
   BK_CHECK(x.is_cuda(), "x must be a GPU tensor");
   block_type(x, "x");
-  return DropoutFn::apply(x, seed, MaskOpts{thr, up, seed_v, offset_v}, wants_grad({x}));
+  return DropoutFn::apply(x, seed, MaskOpts{thr, up, seed_v, offset_v}, wants_grad({x}, x));
 }
 
 // ------------------------------------------------------------------ gated residual norm
@@ -317,7 +331,7 @@ std::vector<Tensor> block_residual(const Tensor& x, const Tensor& y, const OptTe
   return ResidualFn::apply(
       x, y, gate, post_w, post_b, pre_w, pre_b, seed,
       ResidualOpts{post, pre, gate_kind, sigmoid, x_scale, y_scale, eps, {thr, up, seed_v, offset_v}},
-      wants_grad({x, y, gate, post_w, post_b, pre_w, pre_b}));
+      wants_grad({x, y, gate, post_w, post_b, pre_w, pre_b}, x));
 }
 
 // ------------------------------------------------------------------ 8-bit fc
@@ -590,7 +604,7 @@ Tensor block_fp8_fc(const Tensor& x, const Tensor& W, const OptTensor& b) {
   block_type(W, "W");
   fp8_dims(x.size(0), x.size(1));
   fp8_dims(W.size(1), 1);
-  return Fp8FcFn::apply(x, W, b, wants_grad({x, W, b}));
+  return Fp8FcFn::apply(x, W, b, wants_grad({x, W, b}, x));
 }
 
 }  // namespace

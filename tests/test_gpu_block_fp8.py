@@ -259,3 +259,97 @@ def test_fc_captured_step_replays():
         torch.cuda.synchronize()
         for a, c in zip(out, want):
             assert torch.equal(a, c), i
+
+
+@pytest.mark.parametrize("m,n,k", [(3601, 3590, 200), (12700, 1000, 128), (300, 50000, 520)])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_matmul_large_tiles(m, n, k, dt):
+    """Results over 2^23.6 values take 256 x 256 tiles: ragged ones, one block of K, more than one group of exponents."""
+    x, w = values(m, k, seed=6), values(n, k, seed=7)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(3))
+    y = fp8_matmul(fp8_quantize(x.to(DEV)), fp8_quantize(w.to(DEV)), bias.to(DEV), dt)
+    product_near(y, held(x, 1, 128), held(w, 1, 128), bias)
+
+
+@pytest.mark.parametrize("m,k,o", [(65, 500, 40), (4000, 130, 3300)])
+def test_fc_mixed_launches(m, k, o):
+    """dx and dW in one launch, each in slices or not, and apart where one of them takes large tiles."""
+    check_fc(m, k, o, BF16)
+    check_fc(m, k, o, F32)
+
+
+def test_two_graphs_share_nothing():
+    """Two captured steps of one layer replayed in turn and against eager work keep their own temporaries."""
+    W = torch.randn(400, 400, device=DEV)
+    xs = [torch.randn(m, 400, device=DEV) for m in (700, 1300)]
+    want = [scaled_fp8fc(x, W) for x in xs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x in xs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(scaled_fp8fc(x, W))
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+        eager = scaled_fp8fc(xs[0], W)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0]) and all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_capture_beside_a_live_eager_graph_is_refused():
+    """The backward of a captured step may not meet a leaf that an eager graph on the default stream still holds."""
+    W = torch.randn(40, 40, device=DEV).requires_grad_()
+    x = torch.randn(70, 40, device=DEV)
+    alive = scaled_fp8fc(x, W)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        with torch.cuda.graph(g):
+            scaled_fp8fc(x, W)
+    del alive, g
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = scaled_fp8fc(x, W)
+        (dW,) = torch.autograd.grad(y, W, torch.ones_like(y))
+    g.replay()
+    torch.cuda.synchronize()
+    product_near(dW, held(x, 128, 1).t(), torch.ones(40, 70, dtype=torch.float64))
+
+
+def test_block_of_a_tower():
+    """The operators as they are used together: stream, branch -> residual_norm with dropout -> fc -> relu -> fc, forward
+    and backward; each is held to its oracle on what the one before it gave."""
+    from paddlebox_amd.ops.dropout import keep_mask
+    from paddlebox_amd.ops.residual import residual_norm
+
+    from .block_oracle import Residual
+
+    M, D, H = 300, 136, 264
+    g = torch.Generator().manual_seed(1)
+    mk = lambda *s: torch.randn(*s, generator=g).to(DEV).requires_grad_()  # noqa: E731
+    x, y, w, W1, W2, b1 = mk(M, D), mk(M, D), mk(D), mk(D, H), mk(H, D), mk(H)
+    r, h = residual_norm(x, y, y_scale=0.5, post="rms", post_weight=w, pre="rms", pre_weight=w, p=0.25, seed=3, offset=4)
+    a = scaled_fp8fc(h, W1, b1)
+    z = torch.relu(a)
+    out = scaled_fp8fc(z, W2)
+    dout, dr = torch.randn(M, D, generator=g).to(DEV), torch.randn(M, D, generator=g).to(DEV)
+    names = dict(z=z, a=a, h=h, x=x, y=y, w=w, W1=W1, W2=W2, b1=b1)
+    grads = dict(zip(names, torch.autograd.grad((out, r), list(names.values()), (dout, dr))))
+    o = Residual(x, y, x_scale=1.0, y_scale=0.5, gate=None, gate_kind=None, sigmoid=False, post="rms", pre="rms",
+                 w={"post_weight": w, "pre_weight": w}, eps=1e-6, keep=keep_mask((M, D), 16384, None, 3, 4, torch.device("cpu")),
+                 up=4 / 3)
+    near(r, o.r, o.r_mag)
+    near(h, o.h, o.h_mag)
+    product_near(a, held(h, 1, 128), held(W1, 128, 128).t(), b1)
+    product_near(out, held(z, 1, 128), held(W2, 128, 128).t())
+    product_near(grads["z"], held(dout, 1, 128), held(W2, 128, 128))
+    product_near(grads["W2"], held(z, 128, 1).t(), held(dout, 128, 1).t())
+    product_near(grads["h"], held(grads["a"], 1, 128), held(W1, 128, 128))
+    product_near(grads["W1"], held(h, 128, 1).t(), held(grads["a"], 128, 1).t())
+    want = o.backward(dr, grads["h"])
+    near(grads["x"], *want["x"])
+    near(grads["y"], *want["y"])
+    ww, wm = (p + q for p, q in zip(want["pre_weight"], want["post_weight"]))
+    near(grads["w"], ww, wm, roundings=Residual.ROUNDINGS + (M + 64) * 2.0 ** -24)
