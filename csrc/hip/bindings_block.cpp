@@ -109,9 +109,10 @@ class DropoutFn : public torch::autograd::Function<DropoutFn> {
 };
 
 // Whether an autograd node will be recorded for these inputs.  While the
-// stream captures, a leaf whose accumulator an eager graph on the default
-// stream keeps alive is refused: the backward would hand its gradient over to
-// that stream, which may not take part in a capture, and end the process.
+// stream captures, an input that an eager graph on the default stream made, or
+// a leaf whose accumulator such a graph keeps alive, is refused: the backward
+// would hand its gradient over to that stream, which may not take part in a
+// capture, and end the process.
 bool wants_grad(std::initializer_list<OptTensor> ts, const Tensor& like) {
   if (!at::GradMode::is_enabled()) return false;
   bool any = false;
@@ -121,9 +122,9 @@ bool wants_grad(std::initializer_list<OptTensor> ts, const Tensor& like) {
   C10_HIP_CHECK(hipStreamIsCapturing(stream_of(like), &status));
   if (status == hipStreamCaptureStatusNone) return true;
   for (const OptTensor& t : ts) {
-    if (!t.has_value() || !t->requires_grad() || !t->is_leaf()) continue;
-    const auto acc = torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto s = acc ? acc->stream() : c10::nullopt;
+    if (!t.has_value() || !t->requires_grad()) continue;
+    const auto node = t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn();
+    const auto s = node ? node->stream() : c10::nullopt;
     BK_CHECK(!s.has_value() || s->id() != 0,
              "the stream captures a graph while an eager autograd graph of the same leaf is alive; drop its outputs first");
   }
@@ -335,7 +336,7 @@ std::vector<Tensor> block_residual(const Tensor& x, const Tensor& y, const OptTe
 }
 
 // ------------------------------------------------------------------ 8-bit fc
-constexpr int64_t kFp8MaxDim = 65535 * 128;  // tiles of 128 in a launch's second dimension
+constexpr int64_t kFp8MaxDim = 65535 * 128;  // keeps tiles, rows and columns in 32 bits
 
 void fp8_dims(int64_t a, int64_t b) {
   BK_CHECK(a <= kFp8MaxDim && b <= kFp8MaxDim, "fp8: at most ", kFp8MaxDim, " rows or columns");

@@ -63,7 +63,7 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
 template <typename E>
 __global__ __launch_bounds__(256) void k_fp8_quant_rows(Fp8QuantArgs a) {
   const int64_t nb = fp8_kp(a.K) / 128, sp = fp8_sp(a.K);
-  const int64_t blk = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int64_t blk = grid_piece() * 16 + (threadIdx.x >> 4);
   if (blk >= a.M * nb) return;  // the same for the 16 lanes of a block
   const int lane = threadIdx.x & 15;
   const int64_t row = blk / nb, kb = blk % nb, col = kb * 128 + lane * 8;
@@ -889,7 +889,7 @@ template <typename E>
 void quant(const Fp8QuantArgs& a, hipStream_t s) {
   const int64_t kb = fp8_kp(a.K) / 128, mb = fp8_kp(a.M) / 128;
   if (!a.col_codes && !a.slab && !a.tile) {
-    hipLaunchKernelGGL(k_fp8_quant_rows<E>, dim3((unsigned)((a.M * kb + 15) / 16)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(k_fp8_quant_rows<E>, grid_of((a.M * kb + 15) / 16), dim3(256), 0, s, a);
     return;
   }
   hipLaunchKernelGGL(k_fp8_quant_tile<E>, dim3((unsigned)(kb * mb)), dim3(256), 0, s, a);
@@ -902,7 +902,7 @@ int fp8_gemm_ksplit(int M, int N, int64_t K) {
   Fp8GemmArgs g;
   g.M = M;
   g.N = N;
-  if (is_skinny(M, N, K) || is_large(g)) return 1;
+  if (!M || !N || is_skinny(M, N, K) || is_large(g)) return 1;
   return slices(small_tiles(g), K, 256);
 }
 

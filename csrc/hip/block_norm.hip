@@ -30,7 +30,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void k_residual_fwd(ResidualArgs
   const Seed sd = mask_seed(a.mask);
   keep_seed(a.mask, sd);
   const int lane = threadIdx.x % L;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / L;
+  const int64_t row = grid_piece() * kRows + threadIdx.x / L;
   if (row >= a.M) return;  // the same for every thread of a row
   const Columns<L, C, N> at(lane, a.D);
   Vec8<E> y[C];
@@ -159,7 +159,7 @@ void launch_residual_fwd(const ResidualArgs& a, hipStream_t s) {
     constexpr int L = decltype(l)::value, C = decltype(c)::value, rows = L < 256 ? 256 / L : 1;
     by_types(a, [&](auto tr, auto tt) {
       hipLaunchKernelGGL((k_residual_fwd<decltype(tr)::value, decltype(tt)::value, L, C, decltype(n)::value>),
-                         dim3((unsigned)((a.M + rows - 1) / rows)), dim3(L < 256 ? 256 : L), 0, s, a);
+                         grid_of((a.M + rows - 1) / rows), dim3(L < 256 ? 256 : L), 0, s, a);
     });
   });
 }

@@ -37,6 +37,16 @@ void launch_block_cols(const float* slab, int64_t rows, int64_t W, float* const*
 enum NormKind : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
 enum GateKind : int { kGateNone = 0, kGateChannel = 1, kGateRow = 2, kGateFull = 3 };
 
+// A workgroup for each of `wgs` pieces, in two dimensions where one would pass
+// the 2^32 threads that a launch may have there; surplus ones find no piece.
+constexpr int64_t kGridX = 1 << 20;
+inline dim3 grid_of(int64_t wgs) {
+  return wgs <= kGridX ? dim3((unsigned)wgs) : dim3((unsigned)kGridX, (unsigned)((wgs + kGridX - 1) / kGridX));
+}
+#ifdef __HIPCC__
+__device__ __forceinline__ int64_t grid_piece() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+#endif
+
 struct ResidualArgs {
   int64_t M = 0;
   int D = 0;

@@ -307,6 +307,10 @@ def test_capture_beside_a_live_eager_graph_is_refused():
     with pytest.raises(RuntimeError, match="eager autograd graph"):
         with torch.cuda.graph(g):
             scaled_fp8fc(x, W)
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        with torch.cuda.graph(g):
+            scaled_fp8fc(alive, torch.empty(40, 8, device=DEV))
     del alive, g
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
@@ -353,3 +357,22 @@ def test_block_of_a_tower():
     near(grads["y"], *want["y"])
     ww, wm = (p + q for p, q in zip(want["pre_weight"], want["post_weight"]))
     near(grads["w"], ww, wm, roundings=Residual.ROUNDINGS + (M + 64) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("m,n", [(0, 40), (200, 0), (3, 0), (0, 0)])
+def test_empty_products(m, n):
+    a, b = fp8_quantize(torch.randn(m, 600, device=DEV)), fp8_quantize(torch.randn(n, 600, device=DEV))
+    assert fp8_matmul(a, b).shape == (m, n)
+    assert scaled_fp8fc(torch.randn(m, 600, device=DEV), b).shape == (m, n)
+
+
+def test_quantize_more_blocks_than_a_launch_dimension():
+    """2^24 + 8 blocks and more: the grid's second dimension; each row is the row 4096 before it."""
+    part = values(4096, 1025, seed=11).to(BF16).to(DEV)
+    m = 465 * 4096 + 7
+    q, want = fp8_quantize(part.repeat(466, 1)[:m]), fp8_quantize(part)
+    codes, scales = q.codes.view(torch.uint8), want.scales[:, :9]
+    for at in range(0, m, 4096):
+        n = min(4096, m - at)
+        assert torch.equal(codes[at : at + n], want.codes.view(torch.uint8)[:n])
+        assert torch.equal(q.scales[at : at + n, :9], scales[:n])

@@ -367,3 +367,20 @@ def test_captured_step_replays():
 
 def test_low_bits_of_types():
     assert HALF[BF16] == 2.0 ** -8 and HALF[F16] == 2.0 ** -11 and HALF[F32] == 2.0 ** -24
+
+
+def test_more_rows_than_a_launch_dimension():
+    """2^24 + 37 rows of 3: past 2^20 workgroups of 16 rows, forward and backward, against the same rows in a short call."""
+    m, part = (1 << 24) + 37, 1 << 16
+    y = torch.randn(part, 3, device=DEV, dtype=BF16).repeat(m // part + 1, 1)[:m].requires_grad_()
+    x = torch.zeros_like(y).detach()
+    w = torch.ones(3, device=DEV)
+    r, h = residual_norm(x, y, post="rms", post_weight=w, pre="rms", pre_weight=w)
+    (dy,) = torch.autograd.grad(h, y, y.detach().clone())
+    ys = y.detach()[:part].clone().requires_grad_()
+    r1, h1 = residual_norm(x[:part], ys, post="rms", post_weight=w, pre="rms", pre_weight=w)
+    (dy1,) = torch.autograd.grad(h1, ys, ys.detach().clone())
+    for at in range(0, m, part):
+        n = min(part, m - at)
+        for a, b in ((r, r1), (h, h1), (dy, dy1)):
+            assert torch.equal(a[at : at + n], b[:n])
