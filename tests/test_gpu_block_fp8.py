@@ -376,3 +376,22 @@ def test_quantize_more_blocks_than_a_launch_dimension():
         n = min(4096, m - at)
         assert torch.equal(codes[at : at + n], want.codes.view(torch.uint8)[:n])
         assert torch.equal(q.scales[at : at + n, :9], scales[:n])
+
+
+@pytest.mark.parametrize("m", [5, 200])
+@pytest.mark.parametrize("dt", [F32, BF16])
+def test_matmul_outermost_exponent_bytes(m, dt):
+    """Blocks of exponent bytes at both ends, made by hand: what they stand for, NaN for 255."""
+    g = torch.Generator().manual_seed(2)
+    for byte, other in ((0, 227), (1, 227), (254, 27), (255, 127)):
+        # magnitudes 2 .. 3.75 (byte 0, 1: held values of 2^-126 and more) or 1 .. 1.875 (254: finite ones)
+        mag = torch.randint(8, 16, (m, 256), generator=g) / (8 if byte == 254 else 4)
+        a = (mag * (torch.randint(0, 2, (m, 256), generator=g) * 2 - 1)).to(torch.float8_e4m3fn)
+        b = (torch.randint(8, 16, (40, 256), generator=g) / 8).to(torch.float8_e4m3fn)
+        qa = Fp8Blocks(a.to(DEV), torch.full((m, 4), byte, dtype=torch.uint8, device=DEV), 256)
+        qb = Fp8Blocks(b.to(DEV), torch.full((40, 4), other, dtype=torch.uint8, device=DEV), 256)
+        y = fp8_matmul(qa, qb, out_dtype=dt)
+        if byte == 255:
+            assert y.isnan().all() and qa.dequantize().isnan().all()
+        else:
+            product_near(y, qa.dequantize().cpu().double(), qb.dequantize().cpu().double())
