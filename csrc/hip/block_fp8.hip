@@ -8,10 +8,10 @@
 // against a free scale is at most one bit at the small end of the block's
 // range, never precision.  Values that are not finite become NaN codes.
 //
-// Product, results of 16 bits: v_mfma_scale_f32_16x16x128_f8f6f4 takes an
-// exponent byte for each 32 values of either operand; four equal bytes are one
-// block of 128, so the instruction applies the scales with no vector work
-// beside it, and one instruction is exactly one block deep.  Inside the
+// Product, results of 16 bits: v_mfma_scale_f32_16x16x128_f8f6f4 (few rows) and
+// 32x32x64 (tiles) take an exponent byte for each 32 values of either operand;
+// equal bytes are one block of 128, so the instruction applies the scales with
+// no vector work beside it, and a block is one or two of them deep.  Inside the
 // instruction each run of 8 products is aligned to its largest and what lies
 // more than 13 bits below that is dropped (measured; runs are added in full
 // fp32): up to 2^-13 of a run's largest product a value, under the half step
@@ -19,7 +19,8 @@
 // the codes themselves are rounded by.  That is 4.2 PFLOP/s from registers.
 // Results of 32 bits: the codes become bf16 with their scale in registers
 // (v_cvt_scalef32_pk_bf16_fp8; 4 significant bits fit) and go through
-// v_mfma_f32_16x16x32_bf16, which drops nothing above 2^-23 (2.3 PFLOP/s).
+// the bf16 instructions of the same tiles, which drop nothing above 2^-23 (2.3
+// PFLOP/s).
 // A scale holds for all 128 values of its block, so any order of them within
 // the instructions is right as long as both operands use the same.
 #include <hip/hip_runtime.h>
@@ -912,7 +913,10 @@ int fp8_gemm_ksplit(int M, int N, int64_t K) {
   g.M = M;
   g.N = N;
   if (!M || !N || is_skinny(M, N, K) || is_large(g)) return 1;
-  return slices(small_tiles(g), K, 256);
+  // joining slices is a launch of 4 us, about 8 blocks of K: 400 x 400 x 8192 to bf16 takes 34 us whole and 19 in slices,
+  // 512 x 1024 x 1024 8.6 and 11.7
+  const int split = slices(small_tiles(g), K, 256), nb = (int)(fp8_kp(K) / 128);
+  return nb - fp8_slice(nb, split) >= 8 ? split : 1;
 }
 
 bool fp8_gemm_two_split(Fp8GemmArgs& g, Fp8GemmArgs& h) {
