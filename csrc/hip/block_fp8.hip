@@ -8,16 +8,19 @@
 // against a free scale is at most one bit at the small end of the block's
 // range, never precision.  Values that are not finite become NaN codes.
 //
-// Product, results of 16 bits: v_mfma_scale_f32_16x16x128_f8f6f4 (few rows) and
+// Product, bfloat16 results: v_mfma_scale_f32_16x16x128_f8f6f4 (few rows) and
 // 32x32x64 (tiles) take an exponent byte for each 32 values of either operand;
 // equal bytes are one block of 128, so the instruction applies the scales with
 // no vector work beside it, and a block is one or two of them deep.  Inside the
 // instruction each run of 8 products is aligned to its largest and what lies
 // more than 13 bits below that is dropped (measured; runs are added in full
-// fp32): up to 2^-13 of a run's largest product a value, under the half step
-// of a 16-bit result for all but sums that cancel, and far under the 2^-4 that
-// the codes themselves are rounded by.  That is 4.2 PFLOP/s from registers.
-// Results of 32 bits: the codes become bf16 with their scale in registers
+// fp32).  So each of a run's seven other products loses less than 2^-13 of the
+// largest, and a sum at most 7 * 2^-13 = 2^-10.2 of the sum of its runs' largest
+// products: under bfloat16's half step (2^-9 to 2^-8 of a value) unless the sum
+// cancels, and far under the 2^-4 that the codes themselves are rounded by.
+// That is 4.2 PFLOP/s from registers.
+// float32 and float16 results: float16's half step (2^-12 to 2^-11) is smaller
+// than that loss.  The codes become bf16 with their scale in registers
 // (v_cvt_scalef32_pk_bf16_fp8; 4 significant bits fit) and go through
 // the bf16 instructions of the same tiles, which drop nothing above 2^-23 (2.3
 // PFLOP/s).
@@ -359,6 +362,10 @@ __global__ __launch_bounds__(256, 3) void k_fp8_quant_two(Fp8QuantArgs a, Fp8Qua
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+// whether the sums of a result of this type go through the bf16 instructions
+template <typename C>
+constexpr bool kFullSums = !std::is_same<C, __bf16>::value;
+
 // 32 codes of a row, as the instructions take them from a lane.  FULL: as
 // bf16 values with the scale in them; else codes and the exponent byte.
 template <bool FULL>
@@ -497,7 +504,7 @@ struct Fp8Tile {
 // workgroup `wg` of the g.ksplit slices of all tiles
 template <int WR, int WC, int MT, int NT, typename C>
 __device__ __forceinline__ void gemm_tile(const Fp8GemmArgs& g, Fp8Tile<WR, WC, MT, NT>& shared, int wg) {
-  constexpr bool FULL = std::is_same<C, float>::value;
+  constexpr bool FULL = kFullSums<C>;
   using F = Frag<FULL>;
   constexpr int BM = WR * MT * 32, BN = WC * NT * 32, W = WR * WC, ROWS = BM + BN, BLOCK = ROWS * 128;
   auto& lds = shared.lds;
@@ -774,7 +781,7 @@ __global__ __launch_bounds__(256) void k_fp8_finish(Fp8GemmArgs g, Fp8GemmArgs h
 // their sums through LDS in order.
 template <int MT, typename C>
 __global__ __launch_bounds__(512) void k_fp8_skinny(Fp8GemmArgs g) {
-  using F = Frag<std::is_same<C, float>::value>;
+  using F = Frag<kFullSums<C>>;
   constexpr int AHEAD = 3;
   __shared__ f32x4 part[8][MT][64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, fr = lane & 15, fg = lane >> 4;

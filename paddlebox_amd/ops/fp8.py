@@ -127,10 +127,14 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None,
     """a [M, K] times b [N, K] transposed (+ bias [N], float32), accumulated in
     32 bits and rounded once to ``out_dtype``.  Not differentiable.
 
-    On the GPU a 16-bit result comes from the 8-bit matrix instructions, which
+    On the GPU a bfloat16 result comes from the 8-bit matrix instructions, which
     drop, of each run of 8 products along K, what lies more than 13 bits under
-    the run's largest; a float32 result comes from bf16 instructions at half
-    their rate, which do not (held values under 2^-126 count as zero there).
+    the run's largest: a sum is off by at most 7 * 2^-13 of the sum of its runs'
+    largest products, which is under half a step of bfloat16 unless the sum
+    cancels.  float32 and float16 results come from bf16 instructions at half
+    their rate, which drop nothing (held values under 2^-126 count as zero
+    there); ``out_dtype=torch.float32`` is the way to a bfloat16 value of such a
+    sum.
     """
     if a.cols != b.cols:
         raise ValueError(f"fp8_matmul: a has {a.cols} columns, b {b.cols}")
@@ -172,7 +176,9 @@ class _Fp8FcCpu(torch.autograd.Function):
 
 def scaled_fp8fc(x: torch.Tensor, W: Union[torch.Tensor, Fp8Blocks], b: Optional[torch.Tensor] = None) -> torch.Tensor:
     """fc with 8-bit operands: y = q(x) q(W) + b, accumulated in 32 bits and
-    rounded once to x's type.
+    rounded once to x's type.  On the GPU bfloat16 results (y, dx, a bfloat16
+    W's dW) lose in their sums what ``fp8_matmul`` says; a caller whose sums
+    cancel passes ``x.float()``, which has the same codes, and rounds y itself.
 
     x [N, K] and W [K, O]: float32, bfloat16 or float16; b: float32 with O
     values, or None.  x is held in blocks of 128 along K, W in 128 x 128
