@@ -680,12 +680,12 @@ def k_scaled_fp8fc(ctx, op):
 
 
 def _mask_state(ctx, op, device):
-    """The layer's (seed, step) on the step's device."""
+    """The layer's (seed, step) on the step's device: the scope's own tensor,
+    which the layer counts up in place."""
     name = op.inputs["MaskState"][0].name
     st = ctx.scope.get(name)
-    if st.device != device:  # loaded from a file before the first step
-        st = st.to(device)
-        ctx.scope.set(name, st)
+    if st.device != device:  # loaded from a file or initialised by a host executor, before the first step
+        st = ctx.scope._tensors[name] = st.to(device)  # Scope.set copies into the tensor that is there, and keeps it
     return st
 
 

@@ -1,0 +1,112 @@
+"""The (seed, step) state of the fluid layers' dropout masks: where it lives,
+that it moves on wherever it came from, and what each rank draws from it."""
+import numpy as np
+import pytest
+import torch
+
+import paddlebox_amd.fluid as fluid
+from paddlebox_amd.fluid import kernels
+from paddlebox_amd.ps.box_wrapper import BoxWrapper
+from paddlebox_amd.utils.flags import set_flags
+
+from .test_block_fluid import _build
+from .test_fluid import S, _files
+
+STATES = ("b0.mask_state", "b1.mask_state", "drop.mask_state")
+
+
+def _pass(path, device, *, startup, restore=None, save=None, graph=False, k=0, passes=1):
+    """Passes of 10 batches on `device`.  startup: the place that startup runs on, None: it does not run.
+    Returns the scope's parameters and states on the host, and where the states were."""
+    path.mkdir(parents=True, exist_ok=True)
+    set_flags({"FLAGS_padbox_train_steps_per_graph": k})
+    box = fluid.core.BoxWrapper(8, device=device, new=True)
+    try:
+        box.cfg.sgd.mf_create_thresholds = 0.0
+        box.initialize_gpu_and_load_model(slot_vector=list(range(S)), max_keys=200000,
+                                          model_path=str(restore / "sparse") if restore else None)
+        scope = fluid.Scope()
+        main, start, slots, label, dense, loss = _build()
+        main._pipeline_opt = dict(main._pipeline_opt or {}, use_graph=graph)
+        exe = fluid.Executor(fluid.CPUPlace() if device == "cpu" else fluid.CUDAPlace(0))
+        if startup is not None:
+            fluid.Executor(startup).run(start, scope=scope)
+        if restore:
+            fluid.io.load_persistables(exe, str(restore / "dense"), main, scope=scope)
+        ds = fluid.DatasetFactory().create_dataset("PadBoxSlotDataset")
+        ds.set_use_var([label] + slots + [dense])
+        ds.set_batch_size(64)
+        ds.set_filelist(_files(path, 2, 320))
+        ds.disable_shuffle()
+        fluid.core.BoxPS(ds).read_ins_into_memory()
+        boxps = fluid.core.BoxPS(ds)
+        replays = 0
+        for i in range(passes):
+            boxps.begin_pass()
+            stats = exe.train_from_dataset(main, ds, scope=scope, fetch_list=[loss], print_period=1000)
+            replays += stats.get("graph_replays", 0)
+            boxps.end_pass()
+            if save and i == 0:
+                box.save_base(str(save / "sparse"), str(save / "xbox"), "20240101")
+                fluid.io.save_persistables(exe, str(save / "dense"), main, scope=scope)
+        assert (replays > 0) == graph
+        names = [p.name for p in main.all_parameters()] + list(STATES)
+        return ({n: scope.get(n).detach().cpu().numpy().copy() for n in names}, {scope.get(n).device for n in STATES})
+    finally:
+        set_flags({"FLAGS_padbox_train_steps_per_graph": 0})
+        BoxWrapper._instance = None
+
+
+def test_a_state_that_moves_is_the_scopes():
+    """The tensor that a layer reads and counts up is the one that the scope holds and a save writes."""
+    main, startup = fluid.Program(), fluid.Program()
+    with fluid.program_guard(main, startup), fluid.unique_name.guard():
+        x = fluid.layers.data("x", shape=[4], dtype="float32")
+        fluid.contrib.layers.counter_dropout(x, 0.5, seed=3, name="d")
+    scope = fluid.Scope()
+    fluid.Executor(fluid.CPUPlace()).run(startup, scope=scope)
+    op = next(o for o in main.global_block().ops if o.type == "counter_dropout")
+
+    class Ctx:
+        group = None
+
+    Ctx.scope = scope
+    st = kernels._mask_state(Ctx, op, torch.device("meta"))
+    assert st.device.type == "meta" and scope.get("d.mask_state") is st
+    assert kernels._mask_state(Ctx, op, torch.device("meta")) is st
+
+
+def _resume(tmp_path, device, **kw):
+    ck = tmp_path / "ck"
+    want, _ = _pass(tmp_path / "a", device, startup=fluid.CPUPlace() if device == "cpu" else fluid.CUDAPlace(0), passes=2,
+                    save=ck)
+    got, where = _pass(tmp_path / "b", device, startup=None, restore=ck, **kw)
+    assert {d.type for d in where} == {torch.device(device).type}
+    for n in want:
+        if n in STATES:
+            assert got[n][1] == 20 and (got[n] == want[n]).all(), n
+        else:
+            # the bounds of test_block_fluid.py: the CPU's sums alone, the GPU's atomics and codes at a rounding border
+            np.testing.assert_allclose(got[n], want[n], rtol=1e-5 if device == "cpu" else 0,
+                                       atol=1e-6 if device == "cpu" else 1e-4, err_msg=n)
+
+
+def test_resume_without_startup(tmp_path):
+    _resume(tmp_path, "cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(), dict(graph=True, k=1), dict(graph=True, k=4)], ids=["eager", "captured", "captured4"])
+def test_resume_without_startup_gpu(tmp_path, kw):
+    """A checkpoint loaded into an empty scope: its states are host tensors until the first step."""
+    _resume(tmp_path, "cuda:0", **kw)
+
+
+@pytest.mark.gpu
+def test_startup_on_the_host_gpu(tmp_path):
+    """Startup by a host executor, training on the GPU: the masks of a run that started there."""
+    want, _ = _pass(tmp_path / "a", "cuda:0", startup=fluid.CUDAPlace(0))
+    got, where = _pass(tmp_path / "b", "cuda:0", startup=fluid.CPUPlace())
+    assert {d.type for d in where} == {"cuda"}
+    for n in STATES:
+        assert got[n][1] == 10 and (got[n] == want[n]).all(), n
