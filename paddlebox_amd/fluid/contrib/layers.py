@@ -241,8 +241,9 @@ def scaled_fp8fc(input, param_size, param_attr, bias_size, bias_attr, act=None):
 def _mask_state(helper, seed):
     """The persistable (seed, step) a layer's dropout mask is drawn from: the
     step counts the layer's training batches, so a resumed run goes on with
-    the masks of an uninterrupted one.  Without a seed, each layer takes its
-    own from its name."""
+    the masks of an uninterrupted one.  Each rank of a data-parallel job draws
+    masks of its own (the rank is part of the offset); the state is the same on
+    all of them.  Without a seed, each layer takes its own from its name."""
     if seed is None:
         seed = zlib.crc32(helper.name.encode())
     v = helper.block.create_var(f"{helper.name}.mask_state", [2], "int64", persistable=True, stop_gradient=True)
@@ -257,7 +258,7 @@ def _mask_state(helper, seed):
 def counter_dropout(x, dropout_prob, is_test=False, seed=None, name=None,
                     dropout_implementation="downgrade_in_infer"):
     """``fluid.layers.dropout`` with the mask a function of (seed, training
-    step, element), drawn again in the backward and never stored
+    step, rank, element), drawn again in the backward and never stored
     (``ops.dropout.dropout``)."""
     helper = LayerHelper("counter_dropout", name)
     out = helper.create_variable_for_type_inference(x.dtype, x.shape, x.lod_level)

@@ -689,6 +689,25 @@ def _mask_state(ctx, op, device):
     return st
 
 
+def _mask_rank(ctx) -> int:
+    """This process among those that train on other rows of the same step."""
+    import torch.distributed as dist
+
+    return dist.get_rank(ctx.group) if dist.is_available() and dist.is_initialized() else 0
+
+
+def _mask_seed(ctx, st):
+    """(seed, offset) that a rank's mask is drawn from: the step is the offset's
+    low word, the rank its high one.  The state itself is the same on every
+    rank, so a checkpoint of one of them serves all."""
+    rank = _mask_rank(ctx)
+    if rank <= 0:
+        return st
+    own = st.clone()
+    own[1:] += rank << 32
+    return own
+
+
 @kernel("counter_dropout")
 def k_counter_dropout(ctx, op):
     x = ctx.get(op.inputs["X"][0])
@@ -696,7 +715,7 @@ def k_counter_dropout(ctx, op):
     v = v if v.dtype in (torch.float32, torch.bfloat16, torch.float16) else v.float()
     train = ctx.training and not op.attrs.get("is_test")
     st = _mask_state(ctx, op, v.device) if train else None
-    y = dropout_ops.dropout(v, op.attrs["dropout_prob"], st, training=train,
+    y = dropout_ops.dropout(v, op.attrs["dropout_prob"], _mask_seed(ctx, st) if train else None, training=train,
                             mode=op.attrs["dropout_implementation"])
     if train:
         st[1:] += 1  # the backward has the values that this forward read
@@ -713,7 +732,8 @@ def k_fused_residual_norm(ctx, op):
     st = _mask_state(ctx, op, x.device) if drop else None
     r, h = residual_ops.residual_norm(x, y, x_scale=a["x_scale"], y_scale=a["y_scale"], gate=gate,
                                       gate_act=a["gate_act"], post=a["post_norm"], pre=a["pre_norm"], eps=a["epsilon"],
-                                      p=a["dropout_prob"] if drop else 0.0, seed=st, **par)
+                                      p=a["dropout_prob"] if drop else 0.0, seed=_mask_seed(ctx, st) if drop else None,
+                                      **par)
     if drop:
         st[1:] += 1
     ctx.set(op.outputs["R"][0], r)

@@ -1,15 +1,21 @@
 """The (seed, step) state of the fluid layers' dropout masks: where it lives,
 that it moves on wherever it came from, and what each rank draws from it."""
+import os
+
 import numpy as np
 import pytest
 import torch
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 import paddlebox_amd.fluid as fluid
 from paddlebox_amd.fluid import kernels
+from paddlebox_amd.ops.dropout import keep_mask
 from paddlebox_amd.ps.box_wrapper import BoxWrapper
 from paddlebox_amd.utils.flags import set_flags
 
 from .test_block_fluid import _build
+from .test_collective_modes import _port
 from .test_fluid import S, _files
 
 STATES = ("b0.mask_state", "b1.mask_state", "drop.mask_state")
@@ -110,3 +116,82 @@ def test_startup_on_the_host_gpu(tmp_path):
     assert {d.type for d in where} == {"cuda"}
     for n in STATES:
         assert got[n][1] == 10 and (got[n] == want[n]).all(), n
+
+
+def _masks(rank, steps=3, ckpt=None, save=None):
+    """What `rank` draws for the same rows: a kept-or-not mask of counter_dropout and of fused_residual_norm a step."""
+    main, startup = fluid.Program(), fluid.Program()
+    with fluid.program_guard(main, startup), fluid.unique_name.guard():
+        x = fluid.layers.data("x", shape=[16], dtype="float32")
+        d = fluid.contrib.layers.counter_dropout(x, 0.5, seed=5, name="d")
+        r, _ = fluid.contrib.layers.fused_residual_norm(x, x, x_scale=0.0, dropout_prob=0.25, seed=7, pre_norm="none", name="r")
+        loss = fluid.layers.reduce_mean(fluid.layers.fc(d, 1, name="f"))
+        fluid.optimizer.SGD(learning_rate=0.0).minimize(loss)
+    scope, exe = fluid.Scope(), fluid.Executor(fluid.CPUPlace())
+    exe.run(startup, scope=scope)
+    if ckpt:
+        fluid.io.load_persistables(exe, ckpt, main, scope=scope)
+    out = []
+    for _ in range(steps):
+        out += [v != 0 for v in exe.run(main, feed={"x": np.ones((9, 16), np.float32)}, fetch_list=[d, r], scope=scope)]
+    if save and rank == 0:
+        fluid.io.save_persistables(exe, save, main, scope=scope)
+    return out, [scope.get(n).tolist() for n in ("d.mask_state", "r.mask_state")]
+
+
+def _rank_worker(rank, port, path, q):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    try:
+        first = _masks(rank, save=path)
+        dist.barrier()
+        q.put((rank, first, _masks(rank, steps=2, ckpt=path)))
+    finally:
+        dist.barrier()
+        dist.destroy_process_group()
+
+
+def _defined(rank, step):
+    at = step + (rank << 32)
+    return [keep_mask((9, 16), thr, None, seed, at, torch.device("cpu")).numpy() for thr, seed in ((32768, 5), (16384, 7))]
+
+
+def test_each_rank_draws_its_own_masks(tmp_path):
+    """Two data-parallel ranks on the same rows: masks of (seed, step, rank), one state that a checkpoint of rank 0 gives
+    to both, and a resumed run that goes on with each rank's masks."""
+    ctx = mp.get_context("spawn")
+    q, port = ctx.Queue(), _port()
+    ps = [ctx.Process(target=_rank_worker, args=(r, port, str(tmp_path / "ck"), q)) for r in range(2)]
+    for p in ps:
+        p.start()
+    got = {r: v for r, *v in (q.get(timeout=120) for _ in ps)}
+    for p in ps:
+        p.join(timeout=60)
+    for rank, ((first, state), (then, after)) in got.items():
+        assert state == [[5, 3], [7, 3]] and after == [[5, 5], [7, 5]]  # the same on every rank
+        want = [m for step in range(5) for m in _defined(rank, step)]
+        for a, b in zip(first + then, want):
+            np.testing.assert_array_equal(a, b)
+    assert all((a != b).any() for a, b in zip(got[0][0][0], got[1][0][0]))
+
+
+def test_one_process_draws_the_masks_of_rank_0():
+    out, state = _masks(0)
+    assert state == [[5, 3], [7, 3]]
+    for a, b in zip(out, [m for step in range(3) for m in _defined(0, step)]):
+        np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.gpu
+def test_a_later_rank_captured_gpu(tmp_path, monkeypatch):
+    """Rank 1's masks in captured steps are those of its eager steps, and not rank 0's."""
+    zero, _ = _pass(tmp_path / "z", "cuda:0", startup=fluid.CUDAPlace(0))
+    monkeypatch.setattr(kernels, "_mask_rank", lambda ctx: 1)
+    eager, _ = _pass(tmp_path / "e", "cuda:0", startup=fluid.CUDAPlace(0))
+    graphed, _ = _pass(tmp_path / "g", "cuda:0", startup=fluid.CUDAPlace(0), graph=True, k=4)
+    for n in eager:
+        if n in STATES:
+            assert (graphed[n] == eager[n]).all() and (zero[n] == eager[n]).all() and eager[n][1] == 10, n
+        else:
+            np.testing.assert_allclose(graphed[n], eager[n], rtol=0, atol=1e-4, err_msg=n)  # as in test_block_fluid.py
+    assert np.abs(zero["w1"] - eager["w1"]).max() > 1e-3  # other masks train another model
