@@ -727,11 +727,12 @@ def k_fused_residual_norm(ctx, op):
     a = op.attrs
     x, y = (_val(ctx.get(op.inputs[k][0])).float() for k in ("X", "Y"))
     par = {k: ctx.param(op.inputs[k][0]) for k in ("post_weight", "post_bias", "pre_weight", "pre_bias") if op.inputs.get(k)}
-    gate = _val(ctx.get(op.inputs["gate"][0])).float() if op.inputs.get("gate") else None
+    if op.inputs.get("gate"):
+        par["gate"] = _val(ctx.get(op.inputs["gate"][0])).float()
     drop = a["dropout_prob"] > 0 and ctx.training and not a.get("is_test")
     st = _mask_state(ctx, op, x.device) if drop else None
-    r, h = residual_ops.residual_norm(x, y, x_scale=a["x_scale"], y_scale=a["y_scale"], gate=gate,
-                                      gate_act=a["gate_act"], post=a["post_norm"], pre=a["pre_norm"], eps=a["epsilon"],
+    r, h = residual_ops.residual_norm(x, y, x_scale=a["x_scale"], y_scale=a["y_scale"], gate_act=a["gate_act"],
+                                      post=a["post_norm"], pre=a["pre_norm"], eps=a["epsilon"],
                                       p=a["dropout_prob"] if drop else 0.0, seed=_mask_seed(ctx, st) if drop else None,
                                       **par)
     if drop:

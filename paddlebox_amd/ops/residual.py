@@ -21,6 +21,7 @@ from .dropout import Seed, keep_mask, mask_params, upscale
 _KINDS = {"none": 0, "rms": 1, "layer": 2}
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_COLUMNS = 16384
+_NOT_GIVEN = object()  # a gate left out, as against gate=None
 
 
 def _check_norm(name: str, kind: str, weight, bias, D: int, device):
@@ -38,9 +39,9 @@ def _gate_kind(gate, act: str, y: torch.Tensor) -> int:
     """0 none, 1 [D], 2 [..., 1], 3 y's shape."""
     if act not in ("none", "sigmoid"):
         raise ValueError(f"residual_norm: gate_act must be 'none' or 'sigmoid', not {act!r}")
-    if gate is None:
-        if act != "none":
-            raise ValueError("residual_norm: gate_act without a gate")
+    if gate is _NOT_GIVEN and act != "none":
+        raise ValueError("residual_norm: gate_act without a gate")
+    if gate is None or gate is _NOT_GIVEN:
         return 0
     if gate.device != y.device:
         raise ValueError(f"residual_norm: the gate is on {gate.device}, the input on {y.device}")
@@ -68,7 +69,7 @@ def _norm(v, kind, weight, bias, eps):
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor, *, x_scale: float = 1.0, y_scale: float = 1.0,
-                  gate: Optional[torch.Tensor] = None, gate_act: str = "none",
+                  gate: Optional[torch.Tensor] = _NOT_GIVEN, gate_act: str = "none",
                   post: str = "none", post_weight: Optional[torch.Tensor] = None,
                   post_bias: Optional[torch.Tensor] = None,
                   pre: str = "rms", pre_weight: Optional[torch.Tensor] = None,
@@ -84,7 +85,9 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, x_scale: float = 1.0, y_s
     weights and biases are float32 [D].
     ``gate``: None, float32 [D] (a value for each channel), float32 [..., 1]
     (one for each row) or y's shape and type; ``gate_act="sigmoid"`` takes its
-    sigmoid.
+    sigmoid.  A caller whose gate is optional passes ``gate=None`` with its
+    ``gate_act``: no gate, nothing to activate.  ``gate_act`` with the gate left
+    out is refused.
     ``p``, ``seed``, ``offset``: dropout on the normalised branch, as
     ``ops.dropout.dropout`` has it (pass p = 0 at inference).
     Differentiable once, in x, y, gate, weights and biases.
@@ -106,6 +109,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, x_scale: float = 1.0, y_s
     _check_norm("post", post, post_weight, post_bias, D, x.device)
     _check_norm("pre", pre, pre_weight, pre_bias, D, x.device)
     kind = _gate_kind(gate, gate_act, y)
+    if kind == 0:
+        gate, gate_act = None, "none"
     thr, seed_t, seed_v, offset_v = mask_params(p, seed, offset, x.device)
     up = upscale(thr)
     if x.is_cuda:
