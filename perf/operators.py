@@ -318,8 +318,7 @@ def run(s):
     if op == "residual":
         from paddlebox_amd.ops.residual import residual_norm
 
-        r, h = residual_norm(s["x"], s["y"], x_scale=X_SCALE, y_scale=Y_SCALE, gate=s["gate"],
-                             gate_act=case["act"] if s["gate"] is not None else "none",
+        r, h = residual_norm(s["x"], s["y"], x_scale=X_SCALE, y_scale=Y_SCALE, gate=s["gate"], gate_act=case["act"],
                              post=case["post"], post_weight=s["post_weight"], post_bias=s["post_bias"],
                              pre=case["pre"], pre_weight=s["pre_weight"], pre_bias=s["pre_bias"], eps=EPS,
                              p=case["p"], seed=s["seed"])
