@@ -88,3 +88,18 @@ def test_a_bfloat16_input_has_the_codes_of_its_float32():
     a, b = fp8_quantize(x), fp8_quantize(x.float())
     assert torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and torch.equal(a.scales, b.scales)
     product_near(scaled_fp8fc(x.float(), W.float()), held(x, 1, 128), held(W, 128, 128).t())
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 40, 300), (200, 40, 300), (400, 300, 1920), (3601, 3590, 200)])
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+def test_what_is_not_a_number_stays_in_its_row_and_column(m, n, k, dt):
+    """By either route; the other rows and columns keep their values, and the scale of its block comes from the others."""
+    x, w = values(m, k, seed=8), values(n, k, seed=9)
+    x, w = x / x.abs().max(), w / w.abs().max()
+    x[3, k - 10], w[7, 0], w[7, k - 1] = float("inf"), float("nan"), float("-inf")
+    y = fp8_matmul(fp8_quantize(x.to(DEV)), fp8_quantize(w.to(DEV)), out_dtype=dt).cpu()
+    bad = torch.zeros(m, n, dtype=torch.bool)
+    bad[3], bad[:, 7] = True, True
+    assert torch.equal(torch.isnan(y), bad)
+    rows, cols = [i for i in range(min(m, 64)) if i != 3], [i for i in range(n) if i != 7]
+    product_near(y[rows][:, cols], held(x[rows], 1, 128), held(w[cols], 1, 128), exact_runs=dt != BF16)
