@@ -491,10 +491,12 @@ __device__ __forceinline__ void block_barrier() {
 // exponent bytes come by DMA too, the dwords of four blocks at once and four
 // blocks ahead.
 //
-// 8192^3 of random values to bf16 takes 430 to 480 us (2.3 to 2.6 PFLOP/s; the
-// clock falls under this load, constant data take 359), to fp32 826 us (1.33
-// PFLOP/s: bf16 instructions and the conversion beside them).  The matrix
-// instructions and the power they draw bound it.
+// 8192^3 of random values to bf16 takes 430 to 500 us (2.2 to 2.6 PFLOP/s; the
+// clock falls under this load, constant data take 359), to fp32 784 to 826 us and
+// to float16 767 (1.33 to 1.43 PFLOP/s: bf16 instructions and the conversion
+// beside them).  The matrix instructions and the power they draw bound it.  The
+// 256 x 256 form spills 16 registers for 16-bit results, outside its inner loop,
+// and none for fp32.
 template <int WR, int WC, int MT, int NT>
 struct Fp8Tile {
   static constexpr int kThreads = 64 * WR * WC, kRows = (WR * MT + WC * NT) * 32;
@@ -846,9 +848,20 @@ void by_rows(int M, F f) {
   else f(std::integral_constant<int, 4>{});
 }
 
-// Few rows of a go through k_fp8_skinny, one launch that streams b, unless b is large (every workgroup reads a: 48 x
-// 8192 x 8192 takes 34 us there and 27 in tiles with K in slices; 33 x 1024 x 1024 6 against 9) or so narrow that its
-// workgroups are too few for a long K (64 x 64 x 16384: 54 against 18).  Up to 16 rows both take the same time.
+// Few rows of a go through k_fp8_skinny, one launch that streams b, unless b is large (every workgroup reads a) or so
+// narrow that its workgroups are too few for a long K.  Both routes, us, bf16 results, b from memory (rows / tiles with
+// their join; float16 results take up to 3 us more in tiles, the same in rows):
+//    N x K          16 rows       24 rows       32 rows       48 rows       64 rows
+//   1024 x 1024    3.3 /  8.7    3.7 /  8.6    3.9 /  8.5    4.7 /  7.7    5.3 /  8.7
+//   4096 x 4096    9.0 / 14.8   10.7 / 15.2   11.7 / 15.6   14.7 / 16.9   17.5 / 18.0   (N K = 16 M: the last in rows)
+//   4096 x 6144   11.3 / 17.3   12.8 / 17.7   14.0 / 18.0   17.6 / 18.9   21.3 / 19.3
+//   8192 x 4096   14.4 / 16.7   18.9 / 16.8   20.8 / 17.0   27.2 / 17.9   32.5 / 18.4
+//   8192 x 8192   25.5 / 24.5   33.2 / 24.5   36.9 / 24.9   48.5 / 25.7   59.2 / 26.4
+//    512 x 4096    7.8 / 11.7    9.5 / 11.8   10.5 / 12.0   13.5 / 12.1   16.3 / 12.5   (the last K in rows)
+//    512 x 8192   13.2 / 14.5   16.6 / 14.4   18.5 / 14.6   24.0 / 15.1   29.3 / 15.6
+//   1024 x 8192   13.3 / 14.9   16.6 / 15.0   18.6 / 15.3   24.1 / 15.4   29.4 / 15.6   (the last N in rows)
+// The rule is right on both sides of its borders for most of these; it loses up to 56% at 48 rows and 88% at 64 of
+// 1024 x 8192, which a border at a few more columns or by rows times K would mend, and 38% at 24 rows of 4096 x 6144.
 bool is_skinny(int M, int N, int64_t K) {
   if (M > 64 || (N < 1024 && K > 4096)) return false;
   return M <= 16 || (int64_t)N * K <= (int64_t)16 << 20;
@@ -961,8 +974,9 @@ void launch_fp8_quant(const Fp8QuantArgs& a, hipStream_t s) {
 void launch_fp8_quant_two(const Fp8QuantArgs& a, const Fp8QuantArgs& w, hipStream_t s) {
   const bool tiles = a.M && w.M && (a.col_codes || a.tile) && !a.slab && !w.slab;
   const int64_t n = fp8_kp(a.K) / 128 * (fp8_kp(a.M) / 128), m = fp8_kp(w.K) / 128 * (fp8_kp(w.M) / 128);
-  // one launch for both (forward with its quantisers: 8192 x 400 x 400 bf16 15.7 us, two launches 20.2; 16384 x 2048 x
-  // 2048 95 and 98)
+  // one launch for both where the backward wants x^T's codes too (forward with its quantisers: 8192 x 400 x 400 bf16 15.7
+  // us, two launches 20.2; 16384 x 2048 x 2048 95 and 98), though a bf16 x beside an fp32 W then takes the fp32 body's
+  // registers (151 a lane, alone 86); without gradients x goes by rows, in a launch of its own
   if (tiles && by_types(a.t, w.t, [&](auto e, auto f) {
         hipLaunchKernelGGL((k_fp8_quant_two<decltype(e), decltype(f)>), dim3((unsigned)(n + m)), dim3(256), 0, s, a, w, (int)n);
       }))

@@ -35,11 +35,29 @@ __device__ __forceinline__ void norm_back(float g[C][8], const float n[C][8], co
 // LAYER: either norm has a bias, GATE: the gate is one of channels: which sums
 // there are to hold.  With those that are not needed held as well the kernel
 // took 180 registers a lane, one workgroup a CU, and twice the time.  ALL: both
-// norms are there, all of dr, dh, dx and dy wanted, as in training: the
-// conditions on them otherwise fill the scalar registers (32768 x 4096 bf16
-// with ALL 459 us, without 525).  Memory bounds it there: 1.6 GB at 3.5 TB/s,
-// the row's two reductions and their barriers cost the rest; 8192 x 400 fp32
-// with all inputs takes 31 us for 105 MB.
+// norms are there, all of dr, dh, dx and dy wanted: the conditions on them
+// otherwise fill the scalar registers (32768 x 4096 bf16 with a channel gate:
+// with ALL 455 us, without 525).
+//
+// Without a gate, 2^27 elements (us, TB/s of the 6 tensors that are read and
+// written; a large copy 4.8, and up to 8 where some of it lies in the cache):
+//                post rms, pre rms  none, rms       layer, layer    none, layer
+//   bf16  2048   430 (3.8)          355 (4.5)       508 (3.2)       378 (4.3)
+//         4096   359 (4.5)          341 (4.7)       516 (3.1)       391 (4.1)
+//         5120   515 (3.1)          433 (3.7)       793 (2.0)      1043 (1.5)
+//         8192   373 (4.3)          321 (5.0)       566 (2.9)       737 (2.2)
+//        16384  1012 (1.6)         1127 (1.4)      2126 (0.8)      1520 (1.1)
+//   fp32  4096   613 (5.3)          656 (4.9)       680 (4.7)       593 (5.4)
+//         8192   616 (5.2)          589 (5.5)       936 (3.4)      1094 (2.9)
+//        16384  1864 (1.7)         1621 (2.0)      2580 (1.3)      2338 (1.4)
+// and 8192 x 400 fp32 with all inputs and a full gate 30.5 for 105 MB.
+// Up to 4096 columns, and to 8192 without a layer norm, memory bounds it; the
+// row's two reductions and their barriers cost the rest.  At 2049 to 4096
+// columns rms norms alone fit two workgroups of 512 a CU (1 to 15 registers
+// spilled); with a layer norm's bias sums there is one (154 to 173 registers).
+// At 4097 to 8192 columns a layer norm spills 17 to 70 registers, over 8192, two
+// chunks a lane of 1024 threads, every form 85 to 238: what they write and read
+// again is the larger part of the time there.
 template <int TR, int TT, int L, int C, bool N, bool LAYER, bool GATE, bool ALL>
 __global__ __launch_bounds__(L < 256 ? 256 : L, L < 512 ? 2 : L == 512 && !LAYER ? 4 : 1) void k_residual_bwd(ResidualArgs a) {
   using R = typename BlockElem<TR>::type;
@@ -62,6 +80,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L, L < 512 ? 2 : L == 512 && !LAYER
     }
   const bool pre = ALL || (a.pre && a.dh), post = ALL || a.post, has_dr = ALL || a.dr;
   const int pre_kind = LAYER ? a.pre : kNormRms, post_kind = LAYER ? a.post : kNormRms;  // where there is one
+  // all loads of a row in one place, in front of its arithmetic
   struct Raw {
     Vec8<E> y[C], dh[C], gf[C];
     Vec8<R> x[C], dr[C];
