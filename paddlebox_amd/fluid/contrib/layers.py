@@ -16,6 +16,7 @@ import zlib
 
 import numpy as np
 
+from ...ops.dropout import wrap64
 from .. import initializer as I
 from ..framework import ParamAttr
 from ..layer_helper import LayerHelper
@@ -246,12 +247,14 @@ def _mask_state(helper, seed):
     all of them.  Without a seed, each layer takes its own from its name."""
     if seed is None:
         seed = zlib.crc32(helper.name.encode())
+    if isinstance(seed, bool) or not isinstance(seed, (int, np.integer)):
+        raise TypeError(f"{helper.name}: a dropout seed is a whole number, not {seed!r}")
     v = helper.block.create_var(f"{helper.name}.mask_state", [2], "int64", persistable=True, stop_gradient=True)
     sb = helper.startup_program.global_block()
     if not sb.has_var(v.name):
         sv = sb.create_var(v.name, [2], "int64", persistable=True)
         sb.append_op("init_param", outputs={"Out": [sv]},
-                     attrs={"initializer": I.NumpyArrayInitializer(np.array([int(seed), 0], dtype=np.int64))})
+                     attrs={"initializer": I.NumpyArrayInitializer(np.array([wrap64(int(seed)), 0], dtype=np.int64))})
     return v
 
 

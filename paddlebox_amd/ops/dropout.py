@@ -22,7 +22,7 @@ Seed = Union[int, torch.Tensor]
 _LOW = 0xFFFFFFFF
 
 
-def _wrap64(v: int) -> int:
+def wrap64(v: int) -> int:
     """v as a signed 64-bit value with the same bits."""
     v &= (1 << 64) - 1
     return v - (1 << 64) if v >> 63 else v
@@ -50,7 +50,7 @@ def mask_params(p: float, seed: Optional[Seed], offset: int, device: torch.devic
         seed = 0
     if isinstance(seed, bool) or not isinstance(seed, int) or isinstance(offset, bool) or not isinstance(offset, int):
         raise TypeError("dropout: seed and offset must be whole numbers, or seed an int64 tensor [2]")
-    return thr, None, _wrap64(seed), _wrap64(offset)
+    return thr, None, wrap64(seed), wrap64(offset)
 
 
 def upscale(thr: int) -> float:

@@ -195,3 +195,23 @@ def test_a_later_rank_captured_gpu(tmp_path, monkeypatch):
         else:
             np.testing.assert_allclose(graphed[n], eager[n], rtol=0, atol=1e-4, err_msg=n)  # as in test_block_fluid.py
     assert np.abs(zero["w1"] - eager["w1"]).max() > 1e-3  # other masks train another model
+
+
+def test_layer_seeds():
+    """Any whole number is a seed, as for ops.dropout (64 bits of it count); what is not one is refused when the layer is built."""
+    def build(seed):
+        main, startup = fluid.Program(), fluid.Program()
+        with fluid.program_guard(main, startup), fluid.unique_name.guard():
+            x = fluid.layers.data("x", shape=[4], dtype="float32")
+            fluid.contrib.layers.counter_dropout(x, 0.5, seed=seed, name="d")
+            fluid.contrib.layers.fused_residual_norm(x, x, dropout_prob=0.5, seed=seed, name="r")
+        scope = fluid.Scope()
+        fluid.Executor(fluid.CPUPlace()).run(startup, scope=scope)
+        return [scope.get(n).tolist() for n in ("d.mask_state", "r.mask_state")]
+
+    for seed, held in ((0, 0), (-5, -5), (np.int64(7), 7), ((1 << 62) + 12345, (1 << 62) + 12345), (1 << 63, -(1 << 63)),
+                       ((1 << 64) + 3, 3)):
+        assert build(seed) == [[held, 0]] * 2
+    for seed in (1.5, "7", True):
+        with pytest.raises(TypeError, match="whole number"):
+            build(seed)
